@@ -61,6 +61,12 @@ FILE_FLAGS = {
 }
 
 
+# GPU code is compiled without the packed FP32 instructions (v_pk_add/mul/fma_f32, which -O3 forms from
+# ordinary float code): some of their forms have given wrong results on gfx950 now and then. hipcc's host
+# pass does not know the feature and warns; harmless.
+DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
         if cand and Path(cand).exists():
@@ -82,6 +88,10 @@ def _includes() -> list:
 def _flags() -> list:
     return ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"--offload-arch={ARCH}",
             "-Wno-unused-result", "-Wno-unused-command-line-argument"]
+
+
+def _file_flags(src: str) -> list:
+    return (DEVICE_FLAGS if src.endswith(".hip") else []) + FILE_FLAGS.get(src, [])
 
 
 def _headers_digest() -> str:
@@ -116,10 +126,10 @@ def _compile(src: str, force: bool, hdig: str) -> Path:
     with fresh timestamps - or an old object with a new mtime - is judged by what it contains)."""
     s = CSRC / src
     obj = BUILD / (src.replace("/", "__") + ".o")
-    dig = _digest(s.read_bytes(), hdig, hipcc(), _flags(), FILE_FLAGS.get(src, []), _includes())
+    dig = _digest(s.read_bytes(), hdig, hipcc(), _flags(), _file_flags(src), _includes())
     if not force and _stamp_ok(obj, dig):
         return obj
-    cmd = [hipcc()] + _flags() + FILE_FLAGS.get(src, []) + _includes()
+    cmd = [hipcc()] + _flags() + _file_flags(src) + _includes()
     if s.suffix == ".cpp":
         cmd += ["-x", "hip"] if src == "bindings.cpp" else []
     cmd += ["-c", str(s), "-o", str(obj)]
@@ -165,7 +175,7 @@ def _build_hsaco(force: bool, verbose: bool) -> Path:
     out = hsaco_path()
     src = CSRC / "kernels" / "serve_direct.hip"
     cmd = [hipcc(), f"--offload-arch={ARCH}", "--cuda-device-only", "--no-gpu-bundle-output", "-O3", "-std=c++17"] + \
-        _includes() + [str(src), "-o", str(out) + ".tmp"]
+        DEVICE_FLAGS + _includes() + [str(src), "-o", str(out) + ".tmp"]
     dig = _digest(src.read_bytes(), _headers_digest(), cmd[:-3])
     if not force and _stamp_ok(out, dig):
         return out
@@ -210,7 +220,7 @@ def stamp_matches() -> bool:
     for src in SOURCES:
         s = CSRC / src
         obj = BUILD / (src.replace("/", "__") + ".o")
-        d = _digest(s.read_bytes(), hdig, hipcc(), _flags(), FILE_FLAGS.get(src, []), _includes())
+        d = _digest(s.read_bytes(), hdig, hipcc(), _flags(), _file_flags(src), _includes())
         if not _stamp_ok(obj, d):
             return False
         digs.append(d)
