@@ -432,6 +432,66 @@ PYBIND11_MODULE(_C, m) {
       py::arg("params"), py::arg("grad"), py::arg("mom"), py::arg("rows"), py::arg("cols"), py::arg("pen_cols"),
       py::arg("lr"), py::arg("inv_n"), py::arg("l2"), py::arg("momentum"), py::arg("shadow_w"),
       py::arg("shadow_b"), py::arg("stream") = 0);
+  m.attr("LOGIT_MAX_CLASSES") = LOGIT_MAX_CLASSES;
+  m.attr("LOGIT_MAX_TOP") = LOGIT_MAX_TOP;
+  m.def("top_logits_workspace", &top_logits_workspace, py::arg("dt"), py::arg("B"), py::arg("K"), py::arg("k"));
+  m.def(
+      "top_logits",
+      [](int dt, uintptr_t Z, int64_t ldz, int64_t B, int K, int k, uintptr_t values, uintptr_t idx, uintptr_t ws,
+         size_t ws_bytes, uintptr_t stream) {
+        launch_top_logits(dt, ptr<void>(Z), ldz, B, K, k, ptr<void>(values), ptr<int32_t>(idx), ptr<void>(ws), ws_bytes,
+                          stream_of(stream));
+      },
+      py::arg("dt"), py::arg("Z"), py::arg("ldz"), py::arg("B"), py::arg("K"), py::arg("k"), py::arg("values"),
+      py::arg("idx"), py::arg("ws"), py::arg("ws_bytes"), py::arg("stream") = 0);
+  m.def("distill_workspace", &distill_workspace, py::arg("dt"), py::arg("B"), py::arg("K"));
+  m.def(
+      "distill",
+      [](int dt, int t_dt, int out_dt, uintptr_t Z, int64_t ldz, int64_t B, int K, uintptr_t idx, int64_t ldi,
+         uintptr_t t, int64_t ldt, int k, float temperature, float alpha, uintptr_t y, uintptr_t g, uintptr_t stats_in,
+         uintptr_t loss, uintptr_t stats_out, uintptr_t pred, uintptr_t dz, int64_t ldd, uintptr_t ws, size_t ws_bytes,
+         uintptr_t stream) {
+        DistillCall c;
+        c.dt = dt, c.t_dt = t_dt, c.out_dt = out_dt;
+        c.Z = ptr<void>(Z), c.idx = ptr<int32_t>(idx), c.t = ptr<void>(t), c.y = ptr<int32_t>(y), c.g = ptr<float>(g);
+        c.stats_in = ptr<void>(stats_in), c.loss = ptr<float>(loss), c.stats_out = ptr<void>(stats_out);
+        c.pred = ptr<int32_t>(pred), c.dz = ptr<void>(dz);
+        c.B = B, c.ldz = ldz, c.ldi = ldi, c.ldt = ldt, c.ldd = ldd, c.K = K, c.k = k;
+        c.temperature = temperature, c.alpha = alpha;
+        c.workspace = ptr<void>(ws), c.ws_bytes = ws_bytes;
+        launch_distill(c, stream_of(stream));
+      },
+      py::arg("dt"), py::arg("t_dt"), py::arg("out_dt"), py::arg("Z"), py::arg("ldz"), py::arg("B"), py::arg("K"),
+      py::arg("idx"), py::arg("ldi"), py::arg("t"), py::arg("ldt"), py::arg("k"), py::arg("temperature"),
+      py::arg("alpha"), py::arg("y"), py::arg("g"), py::arg("stats_in"), py::arg("loss"), py::arg("stats_out"),
+      py::arg("pred"), py::arg("dz"), py::arg("ldd"), py::arg("ws"), py::arg("ws_bytes"), py::arg("stream") = 0);
+  m.def(
+      "sample_logits",
+      [](int dt, uintptr_t Z, int64_t ldz, int64_t B, int K, uintptr_t u, uintptr_t temperature, float temperature_all,
+         uintptr_t top_k, int top_k_all, uintptr_t top_p, float top_p_all, uintptr_t min_p, float min_p_all,
+         uintptr_t idx, uintptr_t prob, uintptr_t ws, size_t ws_bytes, uintptr_t stream) {
+        SampleCall c;
+        c.dt = dt, c.Z = ptr<void>(Z), c.ldz = ldz, c.B = B, c.K = K, c.u = ptr<float>(u);
+        c.temperature = ptr<float>(temperature), c.temperature_all = temperature_all;
+        c.top_k = ptr<int32_t>(top_k), c.top_k_all = top_k_all;
+        c.top_p = ptr<float>(top_p), c.top_p_all = top_p_all;
+        c.min_p = ptr<float>(min_p), c.min_p_all = min_p_all;
+        c.idx = ptr<int32_t>(idx), c.prob = ptr<float>(prob), c.workspace = ptr<void>(ws), c.ws_bytes = ws_bytes;
+        launch_sample(c, stream_of(stream));
+      },
+      py::arg("dt"), py::arg("Z"), py::arg("ldz"), py::arg("B"), py::arg("K"), py::arg("u"), py::arg("temperature"),
+      py::arg("temperature_all"), py::arg("top_k"), py::arg("top_k_all"), py::arg("top_p"), py::arg("top_p_all"),
+      py::arg("min_p"), py::arg("min_p_all"), py::arg("idx"), py::arg("prob"), py::arg("ws"), py::arg("ws_bytes"),
+      py::arg("stream") = 0);
+  m.def(
+      "sample_workspace",
+      [](int dt, int64_t B, int K, bool row_k, int top_k) {
+        SampleCall c;
+        c.dt = dt, c.B = B, c.K = K, c.top_k_all = top_k;
+        if (row_k) c.top_k = reinterpret_cast<const int32_t*>(&c);  // only whether it is set matters
+        return sample_workspace(c);
+      },
+      py::arg("dt"), py::arg("B"), py::arg("K"), py::arg("row_k"), py::arg("top_k"));
   m.def(
       "cast",
       [](int src_dt, uintptr_t src, int dst_dt, uintptr_t dst, int64_t n, uintptr_t stream) {

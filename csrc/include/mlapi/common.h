@@ -16,7 +16,7 @@ enum Kind : int32_t {
   KIND_OVR = 3,             // p_k = sigmoid(z_k) / sum_j sigmoid(z_j)
 };
 
-enum DType : int32_t { DT_F64 = 0, DT_F32 = 1, DT_BF16 = 2 };
+enum DType : int32_t { DT_F64 = 0, DT_F32 = 1, DT_BF16 = 2, DT_F16 = 3 };
 
 inline size_t dtype_size(int dt) { return dt == DT_F64 ? 8 : dt == DT_F32 ? 4 : 2; }
 

@@ -354,6 +354,66 @@ void launch_sgd_update_2d(float* params, const float* grad, float* momentum_buf,
                           int pen_cols, float lr, float inv_n, float l2, float momentum, uint16_t* shadow_w,
                           float* shadow_b, hipStream_t stream);
 
+// ---- row operators over class logits (top_logits.hip, distill.hip, sample.hip) -------------------
+// Z: [B, K] f32, bf16 or f16 with unit column stride and row stride ldz (elements, any alignment).
+// The order of a row's classes is: larger logit first, then lower class; -inf and NaN are masked.
+// Workspaces need no initialisation and may differ from call to call.
+constexpr int LOGIT_MAX_CLASSES = 1 << 20;
+constexpr int LOGIT_MAX_TOP = 1024;
+
+// The k first classes of every row: values [B, k] in Z's type, idx int32 [B, k]; past the last
+// unmasked class value = -inf, idx = -1.
+size_t top_logits_workspace(int dt, int64_t B, int K, int k);
+void launch_top_logits(int dt, const void* Z, int64_t ldz, int64_t B, int K, int k, void* values, int32_t* idx,
+                       void* workspace, size_t ws_bytes, hipStream_t stream);
+
+// Distillation from a teacher's top logits (formulas: distill.hip). idx int32 [B, k] and t [B, k]
+// with row strides; y int32 [B] or null; g f32 [B] or null (1). Any of loss f32 [B], stats_out
+// (16 bytes per row), pred int32 [B] (first maximum), dz [B, K] may be null. With stats_in (an
+// earlier call's stats_out on the same Z, temperature and alpha) the row sums are not computed again.
+struct DistillCall {
+  int dt = 0, t_dt = 0, out_dt = 0;
+  const void* Z = nullptr;
+  const int32_t* idx = nullptr;
+  const void* t = nullptr;
+  const int32_t* y = nullptr;
+  const float* g = nullptr;
+  const void* stats_in = nullptr;
+  float* loss = nullptr;
+  void* stats_out = nullptr;
+  int32_t* pred = nullptr;
+  void* dz = nullptr;
+  int64_t B = 0, ldz = 0, ldi = 0, ldt = 0, ldd = 0;
+  int K = 0, k = 0;
+  float temperature = 1.f, alpha = 1.f;
+  void* workspace = nullptr;
+  size_t ws_bytes = 0;
+};
+size_t distill_workspace(int dt, int64_t B, int K);
+void launch_distill(const DistillCall& call, hipStream_t stream);
+
+// One class drawn per row (definition: sample.hip): u f32 [B]; each setting a device array [B] or,
+// where that is null, one value for all rows. idx int32 [B] (-1: no class), prob f32 [B].
+struct SampleCall {
+  int dt = 0;
+  const void* Z = nullptr;
+  const float* u = nullptr;
+  const float* temperature = nullptr;
+  const int32_t* top_k = nullptr;
+  const float* top_p = nullptr;
+  const float* min_p = nullptr;
+  float temperature_all = 1.f, top_p_all = 1.f, min_p_all = 0.f;
+  int top_k_all = 0;
+  int64_t B = 0, ldz = 0;
+  int K = 0;
+  int32_t* idx = nullptr;
+  float* prob = nullptr;
+  void* workspace = nullptr;
+  size_t ws_bytes = 0;
+};
+size_t sample_workspace(const SampleCall& call);
+void launch_sample(const SampleCall& call, hipStream_t stream);
+
 // ---- pack.hip ----------------------------------------------------------------------------------
 void launch_cast(int src_dt, const void* src, int dst_dt, void* dst, int64_t n, hipStream_t stream);
 

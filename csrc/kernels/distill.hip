@@ -1,0 +1,546 @@
+// Distillation from a teacher's top logits, forward and backward, over rows of class logits.
+//
+// Per row of K student logits z and k teacher entries (class c_j, logit t_j), temperature T, soft share a:
+//   q_j = exp(t_j / T) / sum_i exp(t_i / T)          p = softmax(z / T), p1 = softmax(z)
+//   loss = a T^2 sum_j q_j (ln q_j - ln p_{c_j}) - (1 - a) ln p1_y
+//   dz_i = g [ a T (p_i - sum_{j: c_j = i} q_j) + (1 - a) (p1_i - [i = y]) ]
+// An entry with a negative class or a logit of -inf is absent; a row without entries (a label below 0)
+// has no soft (hard) part; a row whose logits are all -inf has neither. A listed class that the student
+// masks makes the loss +inf. A class of K or more, in an
+// entry or a label, makes the row's loss and gradient NaN: nothing is read or written there.
+//
+// The gradient is dense (a softmax over K) except at the k + 1 listed classes: the row is streamed
+// with the softmax alone, and the listed classes are written again afterwards with their whole value,
+// computed from logits gathered before the first store (so dz may be z itself). The first entry of a
+// class sums all entries of it, in their order: a class listed twice costs no atomic.
+//
+// Bound by memory: a row is read once and written once, 7 operations per logit and softmax.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <stdexcept>
+
+#include "kernels/logit_rows.h"
+#include "mlapi/common.h"
+#include "mlapi/kernels.h"
+
+namespace mlapi {
+namespace {
+
+using namespace lrow;
+
+// What a row's softmax needs: the maximum, sum exp((z - m) / T), sum exp(z - m), first class of the maximum.
+struct RowStats {
+  float m, st, s1;
+  int arg;
+};
+
+__device__ __forceinline__ float finite_max(float m) { return m == -__builtin_inff() ? 0.f : m; }
+
+struct Args {
+  const void* Z;
+  const int32_t* idx;
+  const void* t;
+  const int32_t* y;
+  const float* g;
+  const RowStats* stats_in;  // [B], or [B][parts] partial ones
+  float* loss;
+  RowStats* stats_out;
+  void* dz;
+  int32_t* pred;
+  int64_t B, ldz, ldi, ldt, ldd;
+  int K, k, parts, t_dt;
+  float T, soft, hard;  // soft = a, hard = 1 - a (0 without labels)
+};
+
+// The listed classes of one row, in LDS: n = k entries, and the label as one more.
+struct Listed {
+  int* cls;     // class, -1: absent
+  float* lq;    // log2 q_j
+  float* z;     // its logit
+  __device__ Listed(unsigned char* lds, int cap) {
+    cls = reinterpret_cast<int*>(lds);
+    lq = reinterpret_cast<float*>(cls + cap);
+    z = lq + cap;
+  }
+  static __host__ __device__ int capacity(int k) { return (k + 1 + 3) / 4 * 4; }
+  static __host__ __device__ size_t bytes(int k) { return (size_t)capacity(k) * 12; }
+};
+
+// Reads the row's entries (one wave): log2 q into lq (-inf: absent), logits into z. Returns Q (1, or 0 without entries; NaN
+// for a class out of range or a teacher's NaN or inf), and the label's weight (0 without one).
+template <class T>
+__device__ void read_listed(const Args& a, int64_t row, int lane, Listed L, float& Q, float& H) {
+  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
+  const int32_t* idx = a.idx + row * a.ldi;
+  auto entry = [&](int j) -> float {
+    const int64_t at = row * a.ldt + j;
+    if (a.t_dt == DT_F32) return static_cast<const float*>(a.t)[at];
+    if (a.t_dt == DT_BF16) return (float)static_cast<const __bf16*>(a.t)[at];
+    return (float)static_cast<const _Float16*>(a.t)[at];
+  };
+  const float ct = 1.44269504088896340736f / a.T;
+  float mt = -__builtin_inff();
+  int bad = 0;
+  for (int j = lane; j < a.k; j += 64) {
+    int c = idx[j];
+    const float x = entry(j);
+    if (c < 0 || x == -__builtin_inff()) c = -1;
+    if (c >= a.K) bad = 1, c = -1;
+    L.cls[j] = c;
+    L.lq[j] = x;
+    L.z[j] = c < 0 ? 0.f : (float)z[c];
+    if (c >= 0) mt = fmaxf(mt, x);
+  }
+  mt = finite_max(wave_max(mt));
+  float s = 0.f;
+  for (int j = lane; j < a.k; j += 64) {
+    const float x = L.cls[j] < 0 ? -__builtin_inff() : (L.lq[j] - mt) * ct;
+    L.lq[j] = x;
+    s += __builtin_amdgcn_exp2f(x);
+  }
+  s = wave_sum(s);
+  const float ls = s == 0.f ? 0.f : __builtin_amdgcn_logf(s);
+  for (int j = lane; j < a.k; j += 64) L.lq[j] -= ls;
+  Q = s == 0.f ? 0.f : s / s;
+  H = 0.f;
+  int c = -1;
+  if (a.hard != 0.f) {
+    c = a.y[row];
+    if (c >= a.K) bad = 1, c = -1;
+    H = c < 0 ? 0.f : a.hard;
+  }
+  if (lane == 0) {
+    L.cls[a.k] = c;
+    L.z[a.k] = c < 0 ? 0.f : (float)z[c];
+    for (int j = a.k + 1; j < Listed::capacity(a.k); ++j) L.cls[j] = -1;
+  }
+  if (__any(bad)) Q = __builtin_nanf("");
+}
+
+// The row's loss (one wave; every lane gets it). Q and H as read_listed gave them.
+__device__ float row_loss(const Args& a, int lane, Listed L, float Q, float H, RowStats r) {
+  if (r.st == 0.f) return Q != Q ? Q : 0.f;  // no class at all
+  const float m = finite_max(r.m);
+  float soft = 0.f;
+  if (a.soft != 0.f) {
+    // T times every term, so that no finite logit overflows in a quotient by T; q as 2^64 q, so that
+    // a q below the type's range still counts against a logit near the type's lowest value
+    const float lst = a.T * __logf(r.st), ln2_T = a.T * 0.693147180559945309f;
+    for (int j = lane; j < a.k; j += 64) {
+      if (L.cls[j] < 0) continue;
+      const float term = L.lq[j] * ln2_T - ((L.z[j] - m) - lst);
+      soft += L.z[j] == -__builtin_inff() ? __builtin_inff()
+                                          : (term * 0x1p-64f) * __builtin_amdgcn_exp2f(L.lq[j] + 64.f);
+    }
+    soft = wave_sum(soft) * (a.soft * a.T);
+  }
+  float loss = soft;
+  if (H != 0.f) loss += H * (__logf(r.s1) - (L.z[a.k] - m));
+  return loss + (Q - Q) + (r.st - r.st);
+}
+
+// Coefficients of the dense part: dz_i = at exp((z_i - m) / T) + a1 exp(z_i - m).
+__device__ __forceinline__ void dense_coeffs(const Args& a, float g, float Q, float H, RowStats r, float& at,
+                                             float& a1) {
+  const bool none = r.st == 0.f;
+  at = none ? (Q - Q) : g * a.soft * a.T * Q / r.st;
+  a1 = none || H == 0.f ? 0.f : g * H / r.s1;
+}
+
+// Whole gradients of the listed classes in [c0, c1), into `out`; classes that another entry writes, or
+// that lie outside, become -1 in `keep`. One wave; L.cls is only read.
+__device__ void listed_grads(const Args& a, int lane, Listed L, float g, float at, float a1, float m, float H,
+                             bool none, int c0, int c1, float* out, int* keep) {
+  const float ct = 1.44269504088896340736f / a.T, c1e = 1.44269504088896340736f;
+  const int cap = Listed::capacity(a.k);
+  for (int j = lane; j <= a.k; j += 64) {
+    const int c = L.cls[j];
+    int mine = c >= c0 && c < c1 ? c : -1;
+    float v = 0.f;
+    if (mine >= 0) {
+      float sum = 0.f;
+      for (int i = 0; i < cap; i += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(L.cls + i);
+        const int oc[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (oc[e] == c) {
+            if (i + e < j) mine = -1;
+            sum += i + e == a.k ? H : a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[i + e]);
+          }
+      }
+      const float d = L.z[j] - m;
+      v = none ? at : at * __builtin_amdgcn_exp2f(d * ct) - g * sum;
+      if (!none && H != 0.f) v += a1 * __builtin_amdgcn_exp2f(d * c1e);
+    }
+    out[j] = v;
+    keep[j] = mine;
+  }
+}
+
+// ---- rows that stay in registers ----------------------------------------------------------------
+// NTR threads share a row and hold NV vectors each of it; one read, one write.
+template <class T, class TO, int NTR, int NV>
+__global__ __launch_bounds__(NTR < 256 ? 256 : NTR) void distill_rows_kernel(Args a) {
+  constexpr int V = Vec<T>::N, NT = NTR < 256 ? 256 : NTR, RPB = NT / NTR;
+  __shared__ float scratch[NT / 64];
+  __shared__ float bcast[RPB][2];
+  extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
+  const int sub = threadIdx.x / NTR, tid = threadIdx.x % NTR, lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * RPB + sub;
+  if (row >= a.B) return;  // whole waves: rows of fewer than a block's threads have one wave, and no barrier
+  const int K = a.K, cap = Listed::capacity(a.k);
+  unsigned char* mine = dyn + (size_t)sub * (cap * 20);
+  Listed L(mine, cap);
+  float* gv = reinterpret_cast<float*>(mine + cap * 12);
+  int* gc = reinterpret_cast<int*>(gv + cap);
+  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
+  typename Vec<T>::type raw[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) raw[v] = load_vec(z, (v * NTR + tid) * V, K);
+  float Q = 0.f, H = 0.f;
+  if (tid < 64) {
+    read_listed<T>(a, row, lane, L, Q, H);
+    if (NTR > 64 && lane == 0) bcast[sub][0] = Q, bcast[sub][1] = H;
+  }
+  auto sync = [] {
+    if constexpr (NTR > 64) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  auto fmax2 = [](float x, float y) { return fmaxf(x, y); };
+  auto add2 = [](float x, float y) { return x + y; };
+  const float ct = 1.44269504088896340736f / a.T, c1 = 1.44269504088896340736f;
+  RowStats r;
+  if (a.stats_in != nullptr) {
+    r = a.stats_in[row];
+  } else {
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < V; ++e) m = fmaxf(m, (float)raw[v][e]);
+    m = block_reduce<NTR>(m, scratch, fmax2);
+    const float mf = finite_max(m);
+    float st = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < V; ++e) st += __builtin_amdgcn_exp2f(((float)raw[v][e] - mf) * ct);
+    if (a.hard != 0.f)
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s1 += __builtin_amdgcn_exp2f(((float)raw[v][e] - mf) * c1);
+    r.m = m;
+    r.st = block_reduce<NTR>(st, scratch, add2);
+    r.s1 = a.hard != 0.f ? block_reduce<NTR>(s1, scratch, add2) : 0.f;
+    r.arg = 0;
+    if (a.pred != nullptr) {
+      int arg = K;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if ((float)raw[v][e] == m) arg = min(arg, (v * NTR + tid) * V + e);
+      r.arg = block_reduce<NTR>(arg, reinterpret_cast<int*>(scratch), [](int x, int y) { return min(x, y); });
+      if (r.arg == K) r.arg = 0;
+    }
+  }
+  sync();
+  if (NTR > 64) Q = bcast[sub][0], H = bcast[sub][1];
+  const float m = finite_max(r.m), g = a.g != nullptr ? a.g[row] : 1.f;
+  float at, a1;
+  dense_coeffs(a, g, Q, H, r, at, a1);
+  if (tid < 64) {
+    if (a.loss != nullptr) {
+      const float loss = row_loss(a, lane, L, Q, H, r);
+      if (lane == 0) a.loss[row] = loss;
+    }
+    if (lane == 0) {
+      if (a.stats_out != nullptr) a.stats_out[row] = r;
+      if (a.pred != nullptr) a.pred[row] = r.arg;
+    }
+    if (a.dz != nullptr) listed_grads(a, lane, L, g, at, a1, m, H, r.st == 0.f, 0, K, gv, gc);
+  }
+  if (a.dz == nullptr) return;
+  TO* dz = static_cast<TO*>(a.dz) + row * a.ldd;
+  typedef TO out_t __attribute__((ext_vector_type(V), aligned(sizeof(TO))));
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int i = (v * NTR + tid) * V;
+    if (i >= K) break;
+    out_t o;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float d = (float)raw[v][e] - m;
+      float x = r.st == 0.f ? at : at * __builtin_amdgcn_exp2f(d * ct);
+      if (a.hard != 0.f) x += a1 * __builtin_amdgcn_exp2f(d * c1);
+      o[e] = (TO)x;
+    }
+    if (i + V <= K) {
+      *reinterpret_cast<out_t*>(dz + i) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (i + e < K) dz[i + e] = o[e];
+    }
+  }
+  sync();
+  for (int j = tid; j <= a.k; j += NTR)
+    if (gc[j] >= 0) dz[gc[j]] = (TO)gv[j];
+}
+
+// ---- rows cut into parts ------------------------------------------------------------------------
+constexpr int PART_THREADS = 256;
+constexpr int MAX_PARTS = 64;
+
+__device__ __forceinline__ void merge_stats(RowStats& x, const RowStats& y, float ct, float c1) {
+  const float m = fmaxf(x.m, y.m), mf = finite_max(m);
+  const float fx = x.m - mf, fy = y.m - mf;
+  x.st = x.st * __builtin_amdgcn_exp2f(fx * ct) + y.st * __builtin_amdgcn_exp2f(fy * ct);
+  x.s1 = x.s1 * __builtin_amdgcn_exp2f(fx * c1) + y.s1 * __builtin_amdgcn_exp2f(fy * c1);
+  x.arg = y.m > x.m || (y.m == x.m && y.arg < x.arg) ? y.arg : x.arg;
+  x.m = m;
+}
+
+// the statistics of one part of a row: [part * len, part * len + len), len a multiple of 256 vectors
+template <class T>
+__global__ __launch_bounds__(PART_THREADS) void distill_parts_kernel(Args a, int len, RowStats* out) {
+  constexpr int V = Vec<T>::N, U = 4, STEP = PART_THREADS * V;
+  __shared__ RowStats part[PART_THREADS / 64];
+  const int64_t row = blockIdx.y;
+  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
+  const int c0 = blockIdx.x * len, c1 = min(a.K, c0 + len);
+  const float ct = 1.44269504088896340736f / a.T, ce = 1.44269504088896340736f;
+  RowStats r{-__builtin_inff(), 0.f, 0.f, 0};
+  for (int base = c0; base < c1; base += U * STEP) {
+    typename Vec<T>::type raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = base + u * STEP + (int)threadIdx.x * V;
+      raw[u] = i < c1 ? load_vec(z, i, c1) : (typename Vec<T>::type)(minus_inf<T>());
+    }
+    float m = r.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) m = fmaxf(m, (float)raw[u][e]);
+    if (m > r.m) {  // rare after the first vectors
+      if (a.pred != nullptr) {
+        r.arg = a.K;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if ((float)raw[u][e] == m) r.arg = min(r.arg, base + u * STEP + (int)threadIdx.x * V + e);
+      }
+      r.st *= __builtin_amdgcn_exp2f((r.m - m) * ct);
+      r.s1 *= __builtin_amdgcn_exp2f((r.m - m) * ce);
+      r.m = m;
+    }
+    const float mf = finite_max(m);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) r.st += __builtin_amdgcn_exp2f(((float)raw[u][e] - mf) * ct);
+    if (a.hard != 0.f)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) r.s1 += __builtin_amdgcn_exp2f(((float)raw[u][e] - mf) * ce);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const RowStats other{__shfl_xor(r.m, o, 64), __shfl_xor(r.st, o, 64), __shfl_xor(r.s1, o, 64),
+                         __shfl_xor(r.arg, o, 64)};
+    merge_stats(r, other, ct, ce);
+  }
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = r;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < PART_THREADS / 64; ++w) merge_stats(r, part[w], ct, ce);
+    out[row * gridDim.x + blockIdx.x] = r;
+  }
+}
+
+// loss, statistics and gradient from a row's (partial) statistics: one block per chunk of `len`
+template <class T, class TO>
+__global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, int len) {
+  constexpr int V = Vec<T>::N, STEP = PART_THREADS * V;
+  __shared__ float bcast[2];
+  extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
+  const int64_t row = blockIdx.y;
+  const int lane = threadIdx.x & 63, cap = Listed::capacity(a.k);
+  const float ct = 1.44269504088896340736f / a.T, ce = 1.44269504088896340736f;
+  Listed L(dyn, cap);
+  float* gv = reinterpret_cast<float*>(dyn + cap * 12);
+  int* gc = reinterpret_cast<int*>(gv + cap);
+  RowStats r = lane < a.parts ? a.stats_in[row * a.parts + lane] : RowStats{-__builtin_inff(), 0.f, 0.f, a.K};
+  if (a.parts > 1) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const RowStats other{__shfl_xor(r.m, o, 64), __shfl_xor(r.st, o, 64), __shfl_xor(r.s1, o, 64),
+                           __shfl_xor(r.arg, o, 64)};
+      merge_stats(r, other, ct, ce);
+    }
+  } else {
+    r = RowStats{__shfl(r.m, 0, 64), __shfl(r.st, 0, 64), __shfl(r.s1, 0, 64), __shfl(r.arg, 0, 64)};
+  }
+  const float m = finite_max(r.m), g = a.g != nullptr ? a.g[row] : 1.f;
+  float Q = 0.f, H = 0.f, at, a1;
+  const int c0 = blockIdx.x * len, c1 = min(a.K, c0 + len);
+  if (threadIdx.x < 64) {
+    read_listed<T>(a, row, lane, L, Q, H);
+    if (lane == 0) bcast[0] = Q, bcast[1] = H;
+    dense_coeffs(a, g, Q, H, r, at, a1);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    if (blockIdx.x == 0) {
+      if (a.loss != nullptr) {
+        const float loss = row_loss(a, lane, L, Q, H, r);
+        if (lane == 0) a.loss[row] = loss;
+      }
+      if (lane == 0) {
+        if (a.stats_out != nullptr) a.stats_out[row] = r;
+        if (a.pred != nullptr) a.pred[row] = r.arg;
+      }
+    }
+    if (a.dz != nullptr) listed_grads(a, lane, L, g, at, a1, m, H, r.st == 0.f, c0, c1, gv, gc);
+  }
+  if (a.dz == nullptr) return;
+  __syncthreads();
+  Q = bcast[0], H = bcast[1];
+  dense_coeffs(a, g, Q, H, r, at, a1);
+  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
+  TO* dz = static_cast<TO*>(a.dz) + row * a.ldd;
+  typedef TO out_t __attribute__((ext_vector_type(V), aligned(sizeof(TO))));
+  for (int i = c0 + (int)threadIdx.x * V; i < c1; i += STEP) {
+    const typename Vec<T>::type raw = load_vec(z, i, c1);
+    out_t o;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float d = (float)raw[e] - m;
+      float x = r.st == 0.f ? at : at * __builtin_amdgcn_exp2f(d * ct);
+      if (a.hard != 0.f) x += a1 * __builtin_amdgcn_exp2f(d * ce);
+      o[e] = (TO)x;
+    }
+    if (i + V <= c1) {
+      *reinterpret_cast<out_t*>(dz + i) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (i + e < c1) dz[i + e] = o[e];
+    }
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j <= a.k; j += PART_THREADS)
+    if (gc[j] >= 0) dz[gc[j]] = (TO)gv[j];
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+template <class T, class TO, int NTR, int NV>
+void launch_rows(const Args& a, hipStream_t stream) {
+  constexpr int NT = NTR < 256 ? 256 : NTR, RPB = NT / NTR;
+  const size_t lds = (size_t)RPB * Listed::capacity(a.k) * 20;
+  hipLaunchKernelGGL((distill_rows_kernel<T, TO, NTR, NV>), dim3((unsigned)((a.B + RPB - 1) / RPB)), dim3(NT), lds,
+                     stream, a);
+  MLAPI_HIP_CHECK(hipGetLastError());
+}
+
+struct Plan {
+  int parts = 0;  // 0: whole rows in registers
+  int len = 0;    // logits per part
+};
+
+template <class T>
+Plan make_plan(int64_t B, int K) {
+  Plan p;
+  (void)B;
+  constexpr int STEP = PART_THREADS * Vec<T>::N;
+  const int steps = (K + STEP - 1) / STEP;
+  if (K <= 64 * 4 * Vec<T>::N) return p;
+  p.parts = std::min(MAX_PARTS, steps);
+  p.len = (steps + p.parts - 1) / p.parts * STEP;
+  p.parts = (K + p.len - 1) / p.len;
+  return p;
+}
+
+template <class T, class TO>
+void run_distill(Args a, RowStats* ws, hipStream_t stream) {
+  const Plan p = make_plan<T>(a.B, a.K);
+  if (p.parts == 0) return launch_rows<T, TO, 64, 4>(a, stream);
+  const size_t lds = (size_t)Listed::capacity(a.k) * 20;
+  a.parts = 1;
+  for (int64_t r0 = 0; r0 < a.B; r0 += 65535) {  // grid.y holds 16 bits
+    Args b = a;
+    const unsigned rows = (unsigned)std::min<int64_t>(65535, a.B - r0);
+    b.Z = static_cast<const T*>(a.Z) + r0 * a.ldz;
+    b.idx = a.idx + r0 * a.ldi;
+    b.t = static_cast<const char*>(a.t) + r0 * a.ldt * (int64_t)dtype_size(a.t_dt);
+    if (a.y) b.y = a.y + r0;
+    if (a.g) b.g = a.g + r0;
+    if (a.loss) b.loss = a.loss + r0;
+    if (a.pred) b.pred = a.pred + r0;
+    if (a.stats_out) b.stats_out = a.stats_out + r0;
+    if (a.dz) b.dz = static_cast<TO*>(a.dz) + r0 * a.ldd;
+    if (a.stats_in) {
+      b.stats_in = a.stats_in + r0;
+    } else {
+      hipLaunchKernelGGL((distill_parts_kernel<T>), dim3((unsigned)p.parts, rows), dim3(PART_THREADS), 0, stream, b,
+                         p.len, ws + r0 * p.parts);
+      b.stats_in = ws + r0 * p.parts;
+      b.parts = p.parts;
+    }
+    // the loss gathers logits of the whole row: where the gradient overwrites them it goes first
+    if (b.dz == b.Z && b.loss != nullptr) {
+      Args l = b;
+      l.dz = nullptr;
+      hipLaunchKernelGGL((distill_chunks_kernel<T, TO>), dim3(1, rows), dim3(PART_THREADS), lds, stream, l, p.len);
+      b.loss = nullptr;
+    }
+    hipLaunchKernelGGL((distill_chunks_kernel<T, TO>), dim3(b.dz == nullptr ? 1u : (unsigned)p.parts, rows),
+                       dim3(PART_THREADS), lds, stream, b, p.len);
+  }
+  MLAPI_HIP_CHECK(hipGetLastError());
+}
+
+}  // namespace
+
+size_t distill_workspace(int dt, int64_t B, int K) {
+  const Plan p = dt == DT_F32 ? make_plan<float>(B, K) : make_plan<__bf16>(B, K);
+  return (size_t)p.parts * (size_t)B * sizeof(RowStats);
+}
+
+void launch_distill(const DistillCall& c, hipStream_t stream) {
+  if (c.B <= 0) return;
+  if (c.K < 1 || c.K > LOGIT_MAX_CLASSES || c.k < 1 || c.k > LOGIT_MAX_TOP)
+    throw std::invalid_argument("distill: 1 <= K <= 2^20 classes, 1 <= k <= 1024 entries");
+  if (!(c.temperature >= 1e-6f && c.temperature <= 1e6f))
+    throw std::invalid_argument("distill: temperature in [1e-6, 1e6]");
+  if (!(c.alpha >= 0.f && c.alpha <= 1.f)) throw std::invalid_argument("distill: alpha in [0, 1]");
+  if (c.ldz < c.K || (c.dz != nullptr && c.ldd < c.K)) throw std::invalid_argument("distill: row stride below K");
+  if (c.alpha != 1.f && c.y == nullptr) throw std::invalid_argument("distill: alpha below 1 needs labels");
+  if (c.stats_in == nullptr && c.ws_bytes < distill_workspace(c.dt, c.B, c.K))
+    throw std::invalid_argument("distill: workspace too small");
+  Args a{};
+  a.Z = c.Z, a.idx = c.idx, a.t = c.t, a.y = c.y, a.g = c.g, a.loss = c.loss, a.dz = c.dz, a.pred = c.pred;
+  a.stats_in = static_cast<const RowStats*>(c.stats_in);
+  a.stats_out = static_cast<RowStats*>(c.stats_out);
+  a.B = c.B, a.ldz = c.ldz, a.ldi = c.ldi, a.ldt = c.ldt, a.ldd = c.ldd;
+  a.K = c.K, a.k = c.k, a.parts = 1, a.t_dt = c.t_dt;
+  a.T = c.temperature, a.soft = c.alpha, a.hard = c.y != nullptr ? 1.f - c.alpha : 0.f;
+  RowStats* ws = static_cast<RowStats*>(c.workspace);
+  if (c.dt == DT_F32 && c.out_dt == DT_F32) return run_distill<float, float>(a, ws, stream);
+  if (c.dt == DT_F32 && c.out_dt == DT_BF16) return run_distill<float, __bf16>(a, ws, stream);
+  if (c.dt == DT_BF16 && c.out_dt == DT_BF16) return run_distill<__bf16, __bf16>(a, ws, stream);
+  if (c.dt == DT_F16 && c.out_dt == DT_F16) return run_distill<_Float16, _Float16>(a, ws, stream);
+  throw std::invalid_argument("distill: logits f32, bf16 or f16; the gradient in their type (bf16 also of f32)");
+}
+
+}  // namespace mlapi

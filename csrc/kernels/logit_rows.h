@@ -1,0 +1,139 @@
+// Device helpers of the row operators over class logits (top_logits.hip, distill.hip, sample.hip):
+// 16-byte row loads at any alignment, reductions over the threads that share a row, the total order
+// of a row's classes, and fixed-point weights.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace mlapi {
+namespace lrow {
+
+// A row is read 16 bytes per lane. Rows of an odd stride start at any element: the type's own
+// alignment is all that is promised, and gfx950 loads and stores 16 bytes from there.
+template <class T>
+struct Vec {
+  static constexpr int N = 16 / (int)sizeof(T);
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
+template <class T>
+__device__ __forceinline__ T minus_inf() {
+  return (T)(-__builtin_inff());
+}
+
+// elements [i, i + N) of a row of K; those past its end read as -inf (a masked class) and are not loaded
+template <class T>
+__device__ __forceinline__ typename Vec<T>::type load_vec(const T* row, int i, int K) {
+  constexpr int N = Vec<T>::N;
+  if (i + N <= K) return *reinterpret_cast<const typename Vec<T>::type*>(row + i);
+  typename Vec<T>::type v;
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = i + e < K ? row[i + e] : minus_inf<T>();
+  return v;
+}
+
+// ---- reductions: every lane of the wave gets the result, always by the same tree ----------------
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return v;
+}
+template <class U>
+__device__ __forceinline__ U wave_sum_int(U v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// inclusive prefix sum over the lanes
+template <class U>
+__device__ __forceinline__ U wave_scan(U v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const U up = __shfl_up(v, o, 64);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+
+// Over a block of NT threads; `scratch` holds NT / 64 values and may be used again after the call.
+template <int NT, class U, class Op>
+__device__ __forceinline__ U block_reduce(U v, U* scratch, Op op) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+  if constexpr (NT > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = scratch[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v = op(v, scratch[w]);
+    __syncthreads();
+  }
+  return v;
+}
+
+// ---- the order of a row's classes: larger logit first, then lower class -------------------------
+// An unsigned key that rises with the logit: -0 as +0; NaN as -inf. Masked classes (-inf, NaN) have
+// KEY_MASKED, every other key is larger.
+constexpr uint32_t KEY_MASKED = 0x007fffffu;
+__device__ __forceinline__ uint32_t order_key(float z) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, z + 0.0f);
+  const uint32_t key = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return z != z ? KEY_MASKED : key;
+}
+__device__ __forceinline__ float key_logit(uint32_t key) {
+  const uint32_t b = key ^ ((key & 0x80000000u) ? 0x80000000u : 0xffffffffu);
+  return __builtin_bit_cast(float, b);
+}
+
+// ---- fixed-point weights ------------------------------------------------------------------------
+// w(z) = 2^42 exp((z - m) / T), rounded, m the row's maximum. Integer sums of these do not depend on
+// their order, so masses found by atomics, by lanes or by blocks agree to the bit, and 2^20 of them
+// stay below 2^63. The step of 2^-42 of the largest weight is what a border between two classes can
+// be off by: the exponential is evaluated in f64 (an f32 one, 2^-24 off, would move a border of 65536
+// rows of 1000 classes often enough to be seen).
+constexpr int WEIGHT_BITS = 42;
+__device__ __forceinline__ uint64_t weight(float z, float m, double c /* log2(e) / T */) {
+  if (z == m) return 1ull << WEIGHT_BITS;  // also T -> 0 and m = inf, where (z - m) / T has no value
+  const double y = ((double)z - (double)m) * c + WEIGHT_BITS;
+  if (!(y > -2.0)) return 0;  // rounds to nothing; NaN too
+  const double n = __builtin_rint(y), f = y - n;
+  // 2^f on [-1/2, 1/2] by its series to the 11th power, sum (f ln 2)^k / k!: the next term is 2^-47 of it
+  double p = 0x1.e8cac7351bb25p-32;
+  p = __builtin_fma(p, f, 0x1.e4cf5158b8ecap-28);
+  p = __builtin_fma(p, f, 0x1.b5253d395e7c4p-24);
+  p = __builtin_fma(p, f, 0x1.62c0223a5c824p-20);
+  p = __builtin_fma(p, f, 0x1.ffcbfc588b0c7p-17);
+  p = __builtin_fma(p, f, 0x1.430912f86c787p-13);
+  p = __builtin_fma(p, f, 0x1.5d87fe78a6731p-10);
+  p = __builtin_fma(p, f, 0x1.3b2ab6fba4e77p-7);
+  p = __builtin_fma(p, f, 0x1.c6b08d704a0c0p-5);
+  p = __builtin_fma(p, f, 0x1.ebfbdff82c58fp-3);
+  p = __builtin_fma(p, f, 0x1.62e42fefa39efp-1);
+  p = __builtin_fma(p, f, 1.0);
+  // the integer nearest to p 2^n falls out of the low bits of a sum with 2^52
+  const double w = __builtin_ldexp(p, (int)n) + 0x1p52;
+  return __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
+}
+
+// floor(u mass) and ceil(p mass) for a fraction 0 <= u, p < 1, exactly
+__device__ __forceinline__ uint64_t fraction_bits(float u) { return (uint64_t)((double)u * 0x1p64); }
+__device__ __forceinline__ uint64_t floor_part(uint64_t mass, float u) { return __umul64hi(mass, fraction_bits(u)); }
+__device__ __forceinline__ uint64_t ceil_part(uint64_t mass, float p) {
+  const uint64_t f = fraction_bits(p);
+  return __umul64hi(mass, f) + (mass * f != 0 ? 1 : 0);
+}
+
+}  // namespace lrow
+}  // namespace mlapi

@@ -1,0 +1,94 @@
+// Selection in the order of a row's classes by one block: the shortest prefix of the order whose
+// count (or mass of fixed-point weights) reaches a target, by histograms in LDS.
+#pragma once
+#include "kernels/logit_rows.h"
+
+namespace mlapi {
+namespace lrow {
+
+// A class's place in the order as one number: the logit's key above, the class counted down below.
+// Larger is earlier, no two classes share one.
+struct Places {
+  int ib;  // bits of a class
+  __device__ explicit Places(int K) : ib(K <= 1 ? 1 : 32 - __builtin_clz((unsigned)(K - 1))) {}
+  __device__ __forceinline__ uint64_t of(uint32_t key, int i) const {
+    return ((uint64_t)key << ib) | (uint64_t)((1u << ib) - 1u - (unsigned)i);
+  }
+  __device__ __forceinline__ uint64_t first(uint32_t key) const { return ((uint64_t)key + 1) << ib; }  // exclusive
+  __device__ __forceinline__ uint64_t last(uint32_t key) const { return (uint64_t)key << ib; }
+  __device__ __forceinline__ int cls(uint64_t place) const {
+    return (int)((1u << ib) - 1u - (unsigned)(place & ((1u << ib) - 1u)));
+  }
+};
+
+struct Prefix {
+  uint64_t cut;    // places >= cut are in it
+  uint64_t count;  // classes in it
+  uint64_t mass;   // their weights
+};
+
+constexpr int SELECT_BINS = 1024;
+struct SelectLds {
+  uint64_t mass[SELECT_BINS];
+  uint32_t count[SELECT_BINS];
+  uint64_t out[4];
+};
+
+// each(f): calls f(place, weight) for every class of this thread with a weight or count to give; all
+// threads of the block together cover the row. target >= 1 and reached by the whole row. The interval
+// of places that holds the target's class is cut into 1024 bins until one class (or an exact end) is
+// left: at most 52 / 10 rounds, one or two for logits without many ties.
+template <int NT, class Each>
+__device__ Prefix select_prefix(bool by_mass, uint64_t target, uint64_t lo, uint64_t hi, SelectLds* s, Each&& each) {
+  uint64_t above_n = 0, above_m = 0;
+  for (;;) {
+    const uint64_t range = hi - lo;
+    const int bits = range == 0 ? 0 : 64 - __builtin_clzll(range);
+    const int sh = bits > 10 ? bits - 10 : 0;
+    __syncthreads();
+    for (int b = threadIdx.x; b < SELECT_BINS; b += NT) s->mass[b] = 0, s->count[b] = 0;
+    __syncthreads();
+    each([&](uint64_t place, uint64_t w) {
+      if (place >= lo && place <= hi) {
+        const int b = (int)((place - lo) >> sh);
+        atomicAdd(&s->count[b], 1u);
+        atomicAdd((unsigned long long*)&s->mass[b], (unsigned long long)w);
+      }
+    });
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      // lane l: bins [16 l, 16 l + 16); the lanes above come first in the order
+      const int l = threadIdx.x;
+      uint64_t n = 0, m = 0;
+      for (int b = 0; b < SELECT_BINS / 64; ++b) n += s->count[l * 16 + b], m += s->mass[l * 16 + b];
+      const uint64_t tn = wave_sum_int(n), tm = wave_sum_int(m);
+      const uint64_t pn = above_n + tn - wave_scan(n, l), pm = above_m + tm - wave_scan(m, l);  // before this lane's
+      const uint64_t before = by_mass ? pm : pn, own = by_mass ? m : n;
+      if (before < target && before + own >= target) {
+        uint64_t cn = pn, cm = pm;
+        for (int b = l * 16 + 15;; --b) {
+          const uint64_t nn = cn + s->count[b], nm = cm + s->mass[b];
+          if ((by_mass ? nm : nn) >= target || b == l * 16) {
+            s->out[0] = b, s->out[1] = cn, s->out[2] = cm;
+            break;
+          }
+          cn = nn, cm = nm;
+        }
+      }
+    }
+    __syncthreads();
+    const int b = (int)s->out[0];
+    above_n = s->out[1], above_m = s->out[2];
+    const uint64_t n = s->count[b], m = s->mass[b];
+    lo += (uint64_t)b << sh;
+    if (sh == 0 || n == 1 || (by_mass ? above_m + m : above_n + n) == target) {
+      __syncthreads();
+      return Prefix{lo, above_n + n, above_m + m};
+    }
+    const uint64_t top = lo + (((uint64_t)1 << sh) - 1);
+    hi = top < hi ? top : hi;
+  }
+}
+
+}  // namespace lrow
+}  // namespace mlapi

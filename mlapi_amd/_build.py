@@ -41,6 +41,9 @@ SOURCES = [
     "kernels/softmax_grad_dw.hip",
     "kernels/softmax_grad_wide.hip",
     "kernels/xcd.hip",
+    "kernels/top_logits.hip",
+    "kernels/distill.hip",
+    "kernels/sample.hip",
     "runtime/engine.cpp",
     "runtime/direct_dispatch.cpp",
     "http/server.cpp",

@@ -1,0 +1,295 @@
+"""Row operators over class logits (top_logits, distill_*, sample_logits) against plain 64-bit forms."""
+import pytest
+import torch
+
+from logits_cases import INF, distill_bounds, rows, teacher
+from mlapi_amd.ops import logits as ops
+from mlapi_amd.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+SHAPES = [(1, 1), (3, 2), (5, 63), (4, 64), (7, 257), (9, 1000), (2, 1025), (3, 2051), (2, 8192), (3, 8200), (2, 33333),
+          (1, 131075)]
+KINDS = ["bell", "ties", "masked", "lowest", "odd", "flat", "steep"]
+
+
+def same(a, b):
+    """Bit equality of values, NaN and signed zeros included."""
+    a, b = a.detach().cpu(), b.detach().cpu()
+    v = {2: torch.int16, 4: torch.int32}[a.element_size()]
+    return a.shape == b.shape and torch.equal(a.view(v), b.view(v))
+
+
+# -------------------------------------------------------------------------------------------- top
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K", SHAPES)
+@pytest.mark.parametrize("k", [1, 8, 65, 300])
+def test_top_logits(dtype, B, K, k):
+    for n, kind in enumerate(KINDS):
+        Z = rows(B, K, dtype, 10 * n + k, kind, pad=(0, 3)[n % 2], device=DEV)
+        val, idx = ops.top_logits(Z, k)
+        rv, ri = ref.top_logits_ref(Z, k)
+        assert torch.equal(idx, ri), kind
+        assert same(val, rv), kind
+
+
+@pytest.mark.parametrize("k", [1000, 1024])
+def test_top_logits_longest_lists(k):
+    for kind in ("bell", "flat", "masked"):
+        for K in (999, 1024, 5000, 40000):
+            Z = rows(3, K, torch.float32, 5, kind, device=DEV)
+            val, idx = ops.top_logits(Z, k)
+            rv, ri = ref.top_logits_ref(Z, k)
+            assert torch.equal(idx, ri) and same(val, rv), (kind, K)
+
+
+@pytest.mark.parametrize("B", [33, 400, 2000])
+def test_top_logits_many_rows(B):
+    Z = rows(B, 1003, torch.bfloat16, 8, "bell", device=DEV)
+    val, idx = ops.top_logits(Z, 16)
+    rv, ri = ref.top_logits_ref(Z, 16)
+    assert torch.equal(idx, ri) and same(val, rv)
+
+
+# ------------------------------------------------------------------------------------ distillation
+def check_distill(Z, idx, t, temperature, alpha, y=None, g=None):
+    kw = dict(temperature=temperature, alpha=alpha, y=y)
+    rl, rd = ref.distill_ref(Z, idx, t, g=g, **kw)
+    tl, td = distill_bounds(Z.cpu(), idx.cpu(), t.cpu(), rl.cpu(), rd.cpu(), temperature=temperature, alpha=alpha,
+                            y=None if y is None else y.cpu(), g=None if g is None else g.cpu())
+    loss, dz = ops.distill_loss_grad(Z, idx, t, g=g, **kw)
+    loss2, stats = ops.distill_loss(Z, idx, t, **kw)
+    dz2 = ops.distill_grad(Z, idx, t, stats, g=g, **kw)
+    for l, d in ((loss, dz), (loss2, dz2)):
+        l, d, el, ed = l.double().cpu(), d.double().cpu(), rl.cpu(), rd.cpu()
+        assert torch.equal(l.isnan(), el.isnan()) and torch.equal(d.isnan(), ed.isnan())
+        ok = el.isnan() | (l == el) | ((l - el).abs() <= tl)
+        assert ok.all(), (l[~ok][:4], el[~ok][:4], tl[~ok][:4])
+        ok = ed.isnan() | (d == ed) | ((d - ed).abs() <= td)
+        assert ok.all(), (d[~ok][:4], ed[~ok][:4], td[~ok][:4], ok.logical_not().nonzero()[:4])
+    return loss, dz
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K", SHAPES)
+@pytest.mark.parametrize("k,temperature,alpha", [(1, 1.0, 1.0), (8, 2.0, 1.0), (33, 0.7, 0.4), (65, 3.0, 0.0)])
+def test_distill(dtype, B, K, k, temperature, alpha):
+    for n, kind in enumerate(["bell", "ties", "masked", "lowest", "flat"]):
+        Z = rows(B, K, dtype, 3 * n + k, kind, pad=(0, 5)[n % 2], device=DEV)
+        idx, t = teacher(Z, k, n, dtype=TYPES[(n + k) % 3], device=DEV)
+        y = g = None
+        if alpha != 1.0:
+            gen = torch.Generator().manual_seed(n)
+            y = torch.randint(-1, K, (B,), generator=gen).to(torch.int32).to(DEV)
+            g = (torch.rand(B, generator=gen) * 2 - 1).to(DEV)
+        check_distill(Z, idx, t, temperature, alpha, y, g)
+
+
+def test_distill_nan_inf_and_classes_out_of_range():
+    for K in (100, 3000, 70000):
+        Z = rows(8, K, torch.float32, 1, "bell", device=DEV)
+        idx, t = teacher(Z, 8, 1, device=DEV)
+        y = torch.zeros(8, dtype=torch.int32, device=DEV)
+        Z[3, 5], Z[4, 7] = float("nan"), INF
+        idx[5, 2], y[6] = K, K + 9
+        t[7, 1] = float("nan")
+        loss, dz = ops.distill_loss_grad(Z, idx, t, temperature=2.0, alpha=0.5, y=y)
+        assert loss[3:].isnan().all() and dz[3:].isnan().all()
+        assert loss[:3].isfinite().all() and dz[:3].isfinite().all()
+        loss, stats = ops.distill_loss(Z, idx, t, temperature=2.0, alpha=0.5, y=y)
+        dz = ops.distill_grad(Z, idx, t, stats, temperature=2.0, alpha=0.5, y=y)
+        assert loss[3:].isnan().all() and dz[3:].isnan().all() and dz[:3].isfinite().all()
+
+
+@pytest.mark.parametrize("K", [500, 5000, 50000])
+def test_distill_gradient_sums_to_zero_and_matches_differences(K):
+    """Both softmaxes sum to one, so a row's gradient sums to zero; and a step along a random direction
+    changes the 64-bit loss by the gradient's product with it."""
+    B, k, T, alpha = 4, 12, 1.7, 0.6
+    Z = rows(B, K, torch.float32, 2, "bell", device=DEV)
+    idx, t = teacher(Z, k, 2, device=DEV)
+    y = torch.randint(0, K, (B,), generator=torch.Generator().manual_seed(1)).to(torch.int32).to(DEV)
+    kw = dict(temperature=T, alpha=alpha, y=y)
+    _, dz = ops.distill_loss_grad(Z, idx, t, **kw)
+    # every element is off by at most (adds + 100) 2^-24 of its two parts, whose sums over a row are 2 (a T + 1 - a)
+    assert (dz.double().sum(1).abs() <= 2 * (alpha * T + 1 - alpha) * 700 * 2.0 ** -24).all()
+    D = torch.randn(B, K, generator=torch.Generator().manual_seed(3), dtype=torch.float64).to(DEV)
+    h = 1e-4
+    up, dn = (ref.distill_ref(Z.double() + s * h * D, idx, t, **kw)[0] for s in (1, -1))
+    slope, want = (dz.double() * D).sum(1), (up - dn) / (2 * h)
+    # third differences: h^2 / 6 times a third derivative below 8 max|D|^3 / T; rounding of dz as above
+    tol = h * h * 8 * D.abs().amax() ** 3 + 700 * 2.0 ** -24 * 2 * T * D.abs().amax()
+    assert ((slope - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("K", [1000, 9000, 150001])
+def test_distill_in_place_and_bf16_out(K):
+    Z = rows(5, K, torch.float32, 4, "bell", pad=7, device=DEV)
+    idx, t = teacher(Z, 20, 4, device=DEV)
+    y = torch.arange(5, dtype=torch.int32, device=DEV)
+    kw = dict(temperature=2.0, alpha=0.5, y=y)
+    loss, dz = ops.distill_loss_grad(Z, idx, t, **kw)
+    wide = torch.full((5, K + 24), 3.0, dtype=torch.bfloat16, device=DEV)
+    l2, d2 = ops.distill_loss_grad(Z, idx, t, out=wide[:, :K], **kw)
+    assert same(d2, dz.to(torch.bfloat16)) and same(l2, loss)
+    assert (wide[:, K:] == 3.0).all()
+    store = torch.empty(5, K + 7, device=DEV).copy_(torch.nn.functional.pad(Z, (0, 7), value=5.0))
+    own = store[:, :K]
+    l3, d3 = ops.distill_loss_grad(own, idx, t, out=own, **kw)
+    assert d3.data_ptr() == own.data_ptr() and same(d3.contiguous(), dz) and same(l3, loss)
+    assert (store[:, K:] == 5.0).all()
+
+
+@pytest.mark.parametrize("K", [40, 3000, 40000])
+def test_distill_pred_is_the_first_maximum(K):
+    for kind in ("bell", "ties", "flat"):
+        Z = rows(6, K, torch.bfloat16, 6, kind, device=DEV)
+        idx, t = teacher(Z, 4, 6, device=DEV)
+        pred = torch.full((6,), -7, dtype=torch.int32, device=DEV)
+        ops.distill_loss_grad(Z, idx, t, pred=pred)
+        assert torch.equal(pred.long(), Z.float().argmax(1)), kind
+
+
+# ---------------------------------------------------------------------------------------- sampling
+def check_sample(Z, u, **kw):
+    idx, prob = ops.sample_logits(Z, u, **kw)
+    ri, rp = ref.sample_ref(Z, u, **kw)
+    assert torch.equal(idx, ri), (idx[idx != ri][:4], ri[idx != ri][:4], kw)
+    # one rounding of the quotient to f32; the masses' own steps are 2^-42 of the largest weight
+    assert ((prob.double() - rp).abs() <= rp * (2.0 ** -24 + 2.0 ** -40) + Z.shape[1] * 2.0 ** -42).all()
+    return idx, prob
+
+
+FILTERS = [dict(), dict(temperature=0.3), dict(top_k=1), dict(top_k=50), dict(top_k=400, temperature=1.4),
+           dict(top_p=0.9), dict(top_p=0.05), dict(min_p=0.1), dict(min_p=1.0), dict(top_p=0.0),
+           dict(top_k=2000, top_p=0.8, min_p=0.02, temperature=0.8), dict(top_k=7, top_p=0.99), dict(temperature=0.0),
+           dict(temperature=1e30), dict(temperature=1e-30)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K", SHAPES)
+@pytest.mark.parametrize("kind", KINDS)
+def test_sample(dtype, B, K, kind):
+    Z = rows(B, K, dtype, 11, kind, pad=3, device=DEV)
+    for n, f in enumerate(FILTERS):
+        u = torch.rand(B, generator=torch.Generator().manual_seed(n)).to(DEV)
+        check_sample(Z, u, **f)
+
+
+def test_sample_settings_per_row():
+    B, K = 60, 1000
+    Z = rows(B, K, torch.float32, 12, "bell", device=DEV)
+    g = torch.Generator().manual_seed(9)
+    r = torch.arange(B)
+    kw = dict(temperature=torch.where(r % 5 == 0, 0.0, 0.3 + torch.rand(B, generator=g)),
+              top_k=torch.where(r % 3 == 0, -1, r * 25).to(torch.int32),
+              top_p=torch.where(r % 4 == 0, 1.5, torch.rand(B, generator=g)),
+              min_p=torch.where(r % 7 == 0, -1.0, 0.1 * torch.rand(B, generator=g)))
+    check_sample(Z, torch.rand(B, generator=g).to(DEV), **{n: v.to(DEV) for n, v in kw.items()})
+
+
+def test_sample_random_numbers_at_their_ends():
+    """Four equal classes: u splits [0, 1) exactly in quarters; 1 and above, NaN and negative are taken in."""
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 1 - 2.0 ** -24, 1.0, 7.0, -1.0, float("nan"), 0.25 - 2.0 ** -26], device=DEV)
+    Z = torch.full((10, 9), -INF, device=DEV)
+    Z[:, [1, 3, 4, 8]] = 2.0
+    idx, prob = ops.sample_logits(Z, u)
+    assert idx.tolist() == [1, 3, 4, 8, 8, 8, 8, 1, 1, 1]
+    assert (prob == 0.25).all()
+
+
+def test_sample_frequencies_follow_the_probabilities():
+    """n draws of one row with u at the n midpoints: every class comes n p times, to within its two ends."""
+    n, K = 4096, 50
+    z = rows(1, K, torch.float32, 3, "bell", device=DEV)
+    idx, _ = ops.sample_logits(z.expand(n, K).contiguous(), (torch.arange(n, device=DEV) + 0.5) / n)
+    got = torch.bincount(idx.long(), minlength=K).double()
+    assert ((got - n * torch.softmax(z[0].double(), 0)).abs() <= 1.0 + 1e-6 * n).all()
+
+
+# ------------------------------------------------------------------- together, captured, elsewhere
+def step(Zt, Zs, y, u):
+    val, idx = ops.top_logits(Zt, 16)
+    loss, dz = ops.distill_loss_grad(Zs, idx, val, temperature=2.0, alpha=0.5, y=y)
+    label, prob = ops.sample_logits(Zs, u, temperature=0.7, top_k=20, top_p=0.9)
+    return val, idx, loss, dz, label, prob
+
+
+@pytest.mark.parametrize("B,K", [(4, 1000), (200, 1000), (3, 50000), (40, 9000)])
+def test_captured_run_matches_eager_on_every_replay(B, K):
+    Zt, Zs = (rows(B, K, torch.float32, s, "bell", device=DEV) for s in (1, 2))
+    y = torch.zeros(B, dtype=torch.int32, device=DEV)
+    u = torch.rand(B, generator=torch.Generator().manual_seed(0)).to(DEV)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(Zt, Zs, y, u)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(Zt, Zs, y, u)
+    for r in range(4):
+        Zt.copy_(rows(B, K, torch.float32, 10 + r, "bell", device=DEV))
+        Zs.copy_(rows(B, K, torch.float32, 20 + r, "bell", device=DEV))
+        for t in got:
+            t.fill_(-3)
+        torch.cuda.synchronize()
+        graph.replay()
+        want = step(Zt, Zs, y, u)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert same(a, b)
+
+
+def test_runs_on_a_side_stream_and_two_at_once():
+    a, b = (rows(64, 20000, torch.float32, s, "bell", device=DEV) for s in (1, 2))
+    y = torch.zeros(64, dtype=torch.int32, device=DEV)
+    u = torch.rand(64, generator=torch.Generator().manual_seed(0)).to(DEV)
+    want = [step(a, b, y, u), step(b, a, y, u)]
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(s1):
+        g1 = step(a, b, y, u)
+    with torch.cuda.stream(s2):
+        g2 = step(b, a, y, u)
+    torch.cuda.synchronize()
+    for got, w in zip((g1, g2), want):
+        for x, v in zip(got, w):
+            assert same(x, v)
+
+
+def test_same_inputs_give_the_same_bits():
+    Z = rows(64, 30000, torch.bfloat16, 5, "ties", device=DEV)
+    y = torch.zeros(64, dtype=torch.int32, device=DEV)
+    u = torch.rand(64, generator=torch.Generator().manual_seed(0)).to(DEV)
+    first = step(Z, Z, y, u)
+    for _ in range(3):
+        for a, b in zip(first, step(Z, Z, y, u)):
+            assert same(a, b)
+
+
+def test_offsets_past_32_bits():
+    """A row beyond 2^31 elements of its buffer: a strided view reads and writes there."""
+    ld = 1 << 30
+    store = torch.empty(3 * ld, dtype=torch.bfloat16, device=DEV)
+    Z = store.as_strided((3, 1000), (ld, 1))
+    src = rows(3, 1000, torch.bfloat16, 7, "bell", device=DEV)
+    Z.copy_(src)
+    val, idx = ops.top_logits(Z, 8)
+    rv, ri = ref.top_logits_ref(src, 8)
+    assert torch.equal(idx, ri) and same(val, rv)
+    u = torch.full((3,), 0.4, device=DEV)
+    assert torch.equal(ops.sample_logits(Z, u)[0], ref.sample_ref(src, u)[0])
+    loss, dz = ops.distill_loss_grad(src, idx, val)
+    l2, d2 = ops.distill_loss_grad(Z, idx, val, out=Z)
+    assert same(l2, loss) and same(d2.contiguous(), dz)
+
+
+def test_empty_batches():
+    Z = torch.empty(0, 50, device=DEV)
+    val, idx = ops.top_logits(Z, 4)
+    assert val.shape == (0, 4) and idx.shape == (0, 4)
+    loss, dz = ops.distill_loss_grad(Z, idx, val)
+    assert loss.shape == (0,) and dz.shape == (0, 50)
+    assert ops.sample_logits(Z, torch.empty(0, device=DEV))[0].shape == (0,)
