@@ -22,15 +22,72 @@ __device__ __forceinline__ T minus_inf() {
   return (T)(-__builtin_inff());
 }
 
+// element i of a row whose address is the same for the wave: 32-bit offsets from a scalar base (64-bit
+// ones cost two registers for every vector of a row)
+template <class T>
+__device__ __forceinline__ T* elem(T* row, int i) {
+  return reinterpret_cast<T*>(reinterpret_cast<char*>(row) + (size_t)((uint32_t)i * (uint32_t)sizeof(T)));
+}
+template <class T>
+__device__ __forceinline__ const T* elem(const T* row, int i) {
+  return reinterpret_cast<const T*>(reinterpret_cast<const char*>(row) + (size_t)((uint32_t)i * (uint32_t)sizeof(T)));
+}
+
 // elements [i, i + N) of a row of K; those past its end read as -inf (a masked class) and are not loaded
 template <class T>
 __device__ __forceinline__ typename Vec<T>::type load_vec(const T* row, int i, int K) {
   constexpr int N = Vec<T>::N;
-  if (i + N <= K) return *reinterpret_cast<const typename Vec<T>::type*>(row + i);
+  if (i + N <= K) return *reinterpret_cast<const typename Vec<T>::type*>(elem(row, i));
   typename Vec<T>::type v;
 #pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = i + e < K ? row[i + e] : minus_inf<T>();
+  for (int e = 0; e < N; ++e) v[e] = i + e < K ? *elem(row, i + e) : minus_inf<T>();
   return v;
+}
+
+// A vector held over several passes of a row in registers. Each pass unpacks it anew (refresh): left
+// alone, the compiler keeps the f32 values of 16-bit types from the first pass, twice the registers.
+template <class T>
+struct Held {
+  typedef uint32_t raw_t __attribute__((ext_vector_type(4)));
+  raw_t raw;
+  __device__ __forceinline__ void load(const T* row, int i) {
+    raw = __builtin_bit_cast(raw_t, *reinterpret_cast<const typename Vec<T>::type*>(elem(row, i)));
+  }
+  __device__ __forceinline__ void load(const T* row, int i, int K) {
+    raw = __builtin_bit_cast(raw_t, load_vec(row, i, K));
+  }
+  __device__ __forceinline__ void mask() { raw = __builtin_bit_cast(raw_t, masked()); }
+  __device__ __forceinline__ void refresh() { asm volatile("" : "+v"(raw)); }
+  __device__ __forceinline__ float operator[](int e) const {
+    typedef T vec_t __attribute__((ext_vector_type(Vec<T>::N)));
+    return (float)__builtin_bit_cast(vec_t, raw)[e];
+  }
+  static __device__ __forceinline__ auto masked() {
+    typedef T vec_t __attribute__((ext_vector_type(Vec<T>::N)));
+    return (vec_t)(minus_inf<T>());
+  }
+};
+
+// A row's NV vectors per thread, NTR threads: vector v of thread t holds classes [(v NTR + t) N, + N), -inf
+// past the row's end. Only one step of NTR vectors can be cut by that end: its guarded loads come once.
+template <class T, int NTR, int NV>
+__device__ __forceinline__ void load_row(Held<T> (&raw)[NV], const T* row, int tid, int K) {
+  constexpr int STEP = NTR * Vec<T>::N;
+  const int whole = K / STEP;  // the same for the wave
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if (v < whole)
+      raw[v].load(row, v * STEP + tid * Vec<T>::N);
+    else
+      raw[v].mask();
+  }
+  if (whole < NV && whole * STEP < K) {
+    Held<T> last;
+    last.load(row, whole * STEP + tid * Vec<T>::N, K);
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (v == whole) raw[v] = last;
+  }
 }
 
 // ---- reductions: every lane of the wave gets the result, always by the same tree ----------------

@@ -122,7 +122,7 @@ def test_native_calls_refuse_before_any_launch(native):
     for kw, what in ((dict(k=0), "entries"), (dict(K=0), "classes"), (dict(temperature=0.0), "temperature"),
                      (dict(temperature=float("nan")), "temperature"), (dict(alpha=1.5), "alpha"),
                      (dict(alpha=0.5), "labels"), (dict(ldz=99), "stride"), (dict(dz=16, ldd=99), "stride"),
-                     (dict(K=5000, ldz=5000, ws_bytes=0), "workspace"), (dict(out_dt=3), "gradient in their type")):
+                     (dict(K=200000, ldz=200000, ws_bytes=0), "workspace"), (dict(out_dt=3), "gradient in their type")):
         with pytest.raises(ValueError, match=what):
             distill(**kw)
     with pytest.raises(ValueError, match="2\\^20"):
