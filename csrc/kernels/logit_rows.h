@@ -90,44 +90,71 @@ __device__ __forceinline__ void load_row(Held<T> (&raw)[NV], const T* row, int t
   }
 }
 
-// ---- reductions: every lane of the wave gets the result, always by the same tree ----------------
+// ---- reductions over a wave: DPP within its rows of 16 lanes, then through scalar registers ---------
+// (a shuffle through LDS costs its latency at each of six steps). The tree is always the same.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {  // lanes without a source read 0
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+  return (int)dpp<CTRL>((uint32_t)v);
+}
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp(uint64_t v) {
+  return (uint64_t)dpp<CTRL>((uint32_t)(v >> 32)) << 32 | dpp<CTRL>((uint32_t)v);
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+__device__ __forceinline__ int lane_value(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ __forceinline__ float lane_value(float v, int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int l) {
+  return (uint64_t)lane_value((uint32_t)(v >> 32), l) << 32 | lane_value((uint32_t)v, l);
+}
+constexpr int ROW_ROR = 0x120, ROW_SHR = 0x110;
+// op over the 16 lanes of a row, to all of them
+template <class U, class Op>
+__device__ __forceinline__ U row_reduce(U v, Op op) {
+  v = op(v, dpp<ROW_ROR + 8>(v));
+  v = op(v, dpp<ROW_ROR + 4>(v));
+  v = op(v, dpp<ROW_ROR + 2>(v));
+  return op(v, dpp<ROW_ROR + 1>(v));
+}
+template <class U, class Op>
+__device__ __forceinline__ U wave_reduce(U v, Op op) {
+  v = row_reduce(v, op);
+  return op(op(lane_value(v, 0), lane_value(v, 16)), op(lane_value(v, 32), lane_value(v, 48)));
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
+  return wave_reduce(v, [](float x, float y) { return fmaxf(x, y); });
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return v;
+  return wave_reduce(v, [](float x, float y) { return x + y; });
 }
 template <class U>
 __device__ __forceinline__ U wave_sum_int(U v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  return wave_reduce(v, [](U x, U y) { return x + y; });
 }
 // inclusive prefix sum over the lanes
 template <class U>
 __device__ __forceinline__ U wave_scan(U v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const U up = __shfl_up(v, o, 64);
-    if (lane >= o) v += up;
-  }
-  return v;
+  v += dpp<ROW_SHR + 1>(v);
+  v += dpp<ROW_SHR + 2>(v);
+  v += dpp<ROW_SHR + 4>(v);
+  v += dpp<ROW_SHR + 8>(v);
+  const U a = lane_value(v, 15), b = lane_value(v, 31), c = lane_value(v, 47);
+  return v + (lane >= 48 ? a + b + c : lane >= 32 ? a + b : lane >= 16 ? a : 0);
 }
 
 // Over a block of NT threads; `scratch` holds NT / 64 values and may be used again after the call.
 template <int NT, class U, class Op>
 __device__ __forceinline__ U block_reduce(U v, U* scratch, Op op) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+  v = wave_reduce(v, op);
   if constexpr (NT > 64) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;

@@ -39,7 +39,7 @@ struct SelectLds {
 // of places that holds the target's class is cut into 1024 bins until one class (or an exact end) is
 // left: at most 52 / 10 rounds, one or two for logits without many ties.
 template <int NT, class Each>
-__device__ Prefix select_prefix(bool by_mass, uint64_t target, uint64_t lo, uint64_t hi, SelectLds* s, Each&& each) {
+__device__ __forceinline__ Prefix select_prefix(bool by_mass, uint64_t target, uint64_t lo, uint64_t hi, SelectLds* s, Each&& each) {
   uint64_t above_n = 0, above_m = 0;
   for (;;) {
     const uint64_t range = hi - lo;
