@@ -58,6 +58,13 @@ struct Held {
   }
   __device__ __forceinline__ void mask() { raw = __builtin_bit_cast(raw_t, masked()); }
   __device__ __forceinline__ void refresh() { asm volatile("" : "+v"(raw)); }
+  // a copy for one pass, where a refresh in place would stand under a condition (and leave a second
+  // copy of the whole row for the other branch)
+  __device__ __forceinline__ Held fresh() const {
+    Held h = *this;
+    h.refresh();
+    return h;
+  }
   __device__ __forceinline__ float operator[](int e) const {
     typedef T vec_t __attribute__((ext_vector_type(Vec<T>::N)));
     return (float)__builtin_bit_cast(vec_t, raw)[e];
@@ -189,26 +196,25 @@ __device__ __forceinline__ float key_logit(uint32_t key) {
 // rows of 1000 classes often enough to be seen).
 constexpr int WEIGHT_BITS = 42;
 __device__ __forceinline__ uint64_t weight(float z, float m, double c /* log2(e) / T */) {
-  if (z == m) return 1ull << WEIGHT_BITS;  // also T -> 0 and m = inf, where (z - m) / T has no value
-  const double y = ((double)z - (double)m) * c + WEIGHT_BITS;
-  if (!(y > -2.0)) return 0;  // rounds to nothing; NaN too
+  // -inf, NaN and all that rounds to nothing end at 2^-16
+  const double y = __builtin_fmax(__builtin_fma((double)z - (double)m, c, (double)WEIGHT_BITS), -16.0);
   const double n = __builtin_rint(y), f = y - n;
-  // 2^f on [-1/2, 1/2] by its series to the 11th power, sum (f ln 2)^k / k!: the next term is 2^-47 of it
-  double p = 0x1.e8cac7351bb25p-32;
-  p = __builtin_fma(p, f, 0x1.e4cf5158b8ecap-28);
-  p = __builtin_fma(p, f, 0x1.b5253d395e7c4p-24);
-  p = __builtin_fma(p, f, 0x1.62c0223a5c824p-20);
-  p = __builtin_fma(p, f, 0x1.ffcbfc588b0c7p-17);
-  p = __builtin_fma(p, f, 0x1.430912f86c787p-13);
-  p = __builtin_fma(p, f, 0x1.5d87fe78a6731p-10);
-  p = __builtin_fma(p, f, 0x1.3b2ab6fba4e77p-7);
-  p = __builtin_fma(p, f, 0x1.c6b08d704a0c0p-5);
-  p = __builtin_fma(p, f, 0x1.ebfbdff82c58fp-3);
+  // 2^f on [-1/2, 1/2]: 1 + f q(f), q of degree 8 through (2^f - 1) / f at nine Chebyshev points,
+  // 2^-44.6 off; exactly 1 at f = 0, so equal logits weigh the same
+  double p = 0x1.b638718fee5a8p-24;
+  p = __builtin_fma(p, f, 0x1.63d136366db24p-20);
+  p = __builtin_fma(p, f, 0x1.ffcb95269d85ap-17);
+  p = __builtin_fma(p, f, 0x1.4308ac85aa947p-13);
+  p = __builtin_fma(p, f, 0x1.5d87fe86f82cdp-10);
+  p = __builtin_fma(p, f, 0x1.3b2ab7181b755p-7);
+  p = __builtin_fma(p, f, 0x1.c6b08d7047e8bp-5);
+  p = __builtin_fma(p, f, 0x1.ebfbdff823cedp-3);
   p = __builtin_fma(p, f, 0x1.62e42fefa39efp-1);
   p = __builtin_fma(p, f, 1.0);
   // the integer nearest to p 2^n falls out of the low bits of a sum with 2^52
   const double w = __builtin_ldexp(p, (int)n) + 0x1p52;
-  return __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
+  const uint64_t k = __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
+  return z == m ? 1ull << WEIGHT_BITS : k;  // also for m = inf, which has no difference to itself
 }
 
 // floor(u mass) and ceil(p mass) for a fraction 0 <= u, p < 1, exactly

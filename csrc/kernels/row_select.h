@@ -28,26 +28,39 @@ struct Prefix {
 };
 
 constexpr int SELECT_BINS = 1024;
+template <int BINS>
 struct SelectLds {
-  uint64_t mass[SELECT_BINS];
-  uint32_t count[SELECT_BINS];
+  uint64_t mass[BINS];
+  uint32_t count[BINS];
   uint64_t out[4];
 };
 
 // each(f): calls f(place, weight) for every class of this thread with a weight or count to give; all
 // threads of the block together cover the row. target >= 1 and reached by the whole row. The interval
-// of places that holds the target's class is cut into 1024 bins until one class (or an exact end) is
-// left: at most 52 / 10 rounds, one or two for logits without many ties.
-template <int NT, class Each>
-__device__ __forceinline__ Prefix select_prefix(bool by_mass, uint64_t target, uint64_t lo, uint64_t hi, SelectLds* s, Each&& each) {
+// of places that holds the target's class is cut into BINS bins until one class (or an exact end) is
+// left: 1024 bins take one or two rounds for logits without many ties. A wave of its own (NT 64) needs no
+// barrier of its block.
+template <int NT, int BINS, class Each>
+__device__ __forceinline__ Prefix select_prefix(bool by_mass, uint64_t target, uint64_t lo, uint64_t hi,
+                                                SelectLds<BINS>* s, Each&& each) {
+  constexpr int PER = BINS / 64, LOG = __builtin_ctz(BINS);
+  const int tid = NT == 64 ? (int)threadIdx.x & 63 : (int)threadIdx.x;
+  auto sync = [] {
+    if constexpr (NT == 64) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  };
   uint64_t above_n = 0, above_m = 0;
   for (;;) {
     const uint64_t range = hi - lo;
     const int bits = range == 0 ? 0 : 64 - __builtin_clzll(range);
-    const int sh = bits > 10 ? bits - 10 : 0;
-    __syncthreads();
-    for (int b = threadIdx.x; b < SELECT_BINS; b += NT) s->mass[b] = 0, s->count[b] = 0;
-    __syncthreads();
+    const int sh = bits > LOG ? bits - LOG : 0;
+    sync();
+    for (int b = tid; b < BINS; b += NT) s->mass[b] = 0, s->count[b] = 0;
+    sync();
     each([&](uint64_t place, uint64_t w) {
       if (place >= lo && place <= hi) {
         const int b = (int)((place - lo) >> sh);
@@ -55,20 +68,20 @@ __device__ __forceinline__ Prefix select_prefix(bool by_mass, uint64_t target, u
         atomicAdd((unsigned long long*)&s->mass[b], (unsigned long long)w);
       }
     });
-    __syncthreads();
-    if (threadIdx.x < 64) {
-      // lane l: bins [16 l, 16 l + 16); the lanes above come first in the order
-      const int l = threadIdx.x;
+    sync();
+    if (tid < 64) {
+      // lane l: bins [PER l, PER l + PER); the lanes above come first in the order
+      const int l = tid;
       uint64_t n = 0, m = 0;
-      for (int b = 0; b < SELECT_BINS / 64; ++b) n += s->count[l * 16 + b], m += s->mass[l * 16 + b];
+      for (int b = 0; b < PER; ++b) n += s->count[l * PER + b], m += s->mass[l * PER + b];
       const uint64_t tn = wave_sum_int(n), tm = wave_sum_int(m);
       const uint64_t pn = above_n + tn - wave_scan(n, l), pm = above_m + tm - wave_scan(m, l);  // before this lane's
       const uint64_t before = by_mass ? pm : pn, own = by_mass ? m : n;
       if (before < target && before + own >= target) {
         uint64_t cn = pn, cm = pm;
-        for (int b = l * 16 + 15;; --b) {
+        for (int b = l * PER + PER - 1;; --b) {
           const uint64_t nn = cn + s->count[b], nm = cm + s->mass[b];
-          if ((by_mass ? nm : nn) >= target || b == l * 16) {
+          if ((by_mass ? nm : nn) >= target || b == l * PER) {
             s->out[0] = b, s->out[1] = cn, s->out[2] = cm;
             break;
           }
@@ -76,13 +89,13 @@ __device__ __forceinline__ Prefix select_prefix(bool by_mass, uint64_t target, u
         }
       }
     }
-    __syncthreads();
+    sync();
     const int b = (int)s->out[0];
     above_n = s->out[1], above_m = s->out[2];
     const uint64_t n = s->count[b], m = s->mass[b];
     lo += (uint64_t)b << sh;
     if (sh == 0 || n == 1 || (by_mass ? above_m + m : above_n + n) == target) {
-      __syncthreads();
+      sync();
       return Prefix{lo, above_n + n, above_m + m};
     }
     const uint64_t top = lo + (((uint64_t)1 << sh) - 1);

@@ -138,7 +138,7 @@ struct BlockTopLds {
       float most[MAX_GROUPS];
       uint16_t group[MAX_GROUPS];
     } g;
-    SelectLds select;
+    SelectLds<SELECT_BINS> select;
   } u;
   uint64_t cand[BLOCK_CAND];
   uint64_t sorted[BLOCK_TOP];
@@ -250,7 +250,7 @@ __device__ __forceinline__ int block_top(const T* z, int c0, int c1, Places plac
       }
     };
     // more than k classes reach the bound, so the k-th place exists
-    const uint64_t cut = select_prefix<TOP_THREADS>(false, k, bound, ~(uint64_t)0 >> (32 - places.ib),
+    const uint64_t cut = select_prefix<TOP_THREADS, SELECT_BINS>(false, k, bound, ~(uint64_t)0 >> (32 - places.ib),
                                                     &s->u.select, each).cut;
     __syncthreads();
     if (tid == 0) s->n = 0;

@@ -12,13 +12,19 @@
 // Masked classes (-inf, NaN) are never drawn; a row without any other gives class -1, prob 0.
 //
 // Masses are integer sums of fixed-point weights (logit_rows.h), so a draw does not depend on how the
-// row is cut over threads.
+// row is cut over threads. What the filters keep is a prefix of the order, given by its last class (Keep).
+//
+// Which kernel draws a row:
+//   rows of up to 2048 classes: one wave, from registers (sample_wave_kernel);
+//   longer rows with a short top-k: the k first classes by one pass (row_top.h), few long rows in parts;
+//   longer rows else: one block, from registers, two passes of weights (sample_row_kernel);
+//   rows that registers do not hold: one block, from memory (sample_long_kernel).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <stdexcept>
 
-#include "kernels/row_select.h"
+#include "kernels/row_top.h"
 #include "mlapi/common.h"
 #include "mlapi/kernels.h"
 
@@ -49,10 +55,432 @@ __device__ __forceinline__ uint64_t least_weight(float min_p) {
   return (uint64_t)__builtin_ceil((double)fminf(min_p, 1.f) * (double)(1ull << WEIGHT_BITS));
 }
 
-template <class T, int NT>
-__global__ __launch_bounds__(NT) void sample_block_kernel(SampleCall a) {
-  constexpr int V = Vec<T>::N, STEP = NT * V, MAX_STEPS = NT == 1024 ? LOGIT_MAX_CLASSES / STEP : 8;
-  __shared__ SelectLds sel;
+// What is left of a row after top-k and top-p: the classes up to one in the order, and a least weight.
+struct Keep {
+  float m;
+  double c;
+  float z;  // the last class kept: its logit and its number
+  int cls;
+  uint64_t least;
+  __device__ __forceinline__ uint64_t mass(float x, int i) const {
+    const uint64_t w = weight(x, m, c);
+    return (x > z || (x == z && i <= cls)) && w >= least ? w : 0;
+  }
+  __device__ __forceinline__ void upto(uint64_t place, Places places) {
+    z = key_logit((uint32_t)(place >> places.ib));
+    cls = places.cls(place);
+  }
+};
+
+__device__ __forceinline__ Keep keep_all(float m, const Settings& set) {
+  return Keep{m, 1.4426950408889634074 / (double)set.T, -__builtin_inff(), 0x7fffffff, least_weight(set.min_p)};
+}
+
+// ---- from a sorted list ---------------------------------------------------------------------------
+// The draw among the first n classes of a row, sorted places in LDS, by one wave; top-k is done. `w` and
+// `c` hold n entries.
+template <int MAX>
+__device__ __forceinline__ void draw_from_list(const SampleCall& a, int64_t row, const Settings& set, Places places,
+                               const uint64_t* sorted, int n, int lane, uint64_t* w, int* c) {
+  constexpr int PER = MAX / 64;
+  const Keep keep = keep_all(key_logit((uint32_t)(sorted[0] >> places.ib)), set);
+  uint64_t own[PER], mass = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = i * 64 + lane;
+    own[i] = r < n ? weight(key_logit((uint32_t)(sorted[r] >> places.ib)), keep.m, keep.c) : 0;
+    mass += own[i];
+  }
+  const uint64_t target = set.top_p < 1.f ? ceil_part(wave_sum_int(mass), fmaxf(set.top_p, 0.f)) : ~(uint64_t)0;
+  uint64_t before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = i * 64 + lane;
+    const uint64_t upto = before + wave_scan(own[i], lane);
+    before = lane_value(upto, 63);
+    const bool in = r == 0 || upto - own[i] < target;
+    own[i] = in && own[i] >= keep.least ? own[i] : 0;
+    total += own[i];
+    if (r < n) w[r] = own[i], c[r] = places.cls(sorted[r]);
+  }
+  total = wave_sum_int(total);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const uint64_t t = floor_part(total, uniform(a, row));
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (i * 64 >= n) break;
+    const int r = i * 64 + lane, mine = r < n ? c[r] : -1;
+    uint64_t lower = 0;  // the kept mass of lower classes
+    for (int j = 0; j < n; ++j) lower += c[j] < mine ? w[j] : 0;
+    if (own[i] != 0 && lower <= t && t < lower + own[i]) {
+      a.idx[row] = mine;
+      a.prob[row] = (float)((double)own[i] / (double)total);
+    }
+  }
+}
+
+__device__ __forceinline__ void write_one(const SampleCall& a, int64_t row, int cls, float prob) {
+  a.idx[row] = cls;
+  a.prob[row] = prob;
+}
+
+// ---- one wave, row in registers -------------------------------------------------------------------
+constexpr int WAVE_BINS = 256;
+struct WaveLds {
+  union {
+    struct {
+      WaveTopLds top;
+      uint64_t w[WAVE_TOP];
+      int c[WAVE_TOP];
+    } l;
+    SelectLds<WAVE_BINS> select;
+  } u;
+};
+
+// ALL: the call has neither top-k nor top-p
+template <class T, int NV, bool ALL>
+__global__ __launch_bounds__(256) void sample_wave_kernel(SampleCall a) {
+  constexpr int V = Vec<T>::N;
+  __shared__ WaveLds lds[ALL ? 1 : 4];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  if (row >= a.B) return;
+  const int K = a.K;
+  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
+  Held<T> raw[NV];
+  load_row<T, 64, NV>(raw, z, lane, K);
+  const Settings set = settings(a, row);
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < V; ++e) m = fmaxf(m, raw[v][e]);
+  m = wave_max(m);
+  auto pass = [&](auto f) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const Held<T> h = raw[v].fresh();
+#pragma unroll
+      for (int e = 0; e < V; ++e) f(h[e], (v * 64 + lane) * V + e);
+    }
+  };
+  if (m == -__builtin_inff() || !(set.T > 0.f)) {
+    int first = K;
+    pass([&](float x, int i) { first = x == m ? min(first, i) : first; });
+    first = wave_reduce(first, [](int x, int y) { return min(x, y); });
+    const bool none = m == -__builtin_inff();
+    if (lane == 0) write_one(a, row, none ? -1 : first, none ? 0.f : 1.f);
+    return;
+  }
+  Keep keep = keep_all(m, set);
+  if constexpr (!ALL) {
+    WaveLds& s = lds[wave];
+    const Places places(K);
+    if (set.top_k > 0 && set.top_k <= WAVE_TOP) {
+      const int n = wave_top<T, NV>(raw, lane, K, set.top_k, &s.u.l.top);
+      draw_from_list<WAVE_TOP>(a, row, set, places, s.u.l.top.sorted, n, lane, s.u.l.w, s.u.l.c);
+      return;
+    }
+    auto each = [&](auto f) {
+      pass([&](float x, int i) {
+        const uint32_t key = order_key(x);
+        if (key > KEY_MASKED) f(places.of(key, i), weight(x, m, keep.c));
+      });
+    };
+    uint64_t lo = places.last(KEY_MASKED + 1);
+    const uint64_t hi = places.first(order_key(m)) - 1;
+    uint64_t mass = 0;
+    bool cut = false;
+    if (set.top_k > 0 && set.top_k < K) {
+      int valid = 0;
+      pass([&](float x, int) { valid += __popcll(__ballot(x > -__builtin_inff())); });
+      if (set.top_k < valid) {
+        const Prefix p = select_prefix<64, WAVE_BINS>(false, set.top_k, lo, hi, &s.u.select, each);
+        lo = p.cut, mass = p.mass, cut = true;
+      }
+    }
+    if (set.top_p < 1.f) {
+      if (!cut) {
+        each([&](uint64_t, uint64_t w) { mass += w; });
+        mass = wave_sum_int(mass);
+      }
+      const uint64_t target = ceil_part(mass, fmaxf(set.top_p, 0.f));
+      lo = select_prefix<64, WAVE_BINS>(true, target == 0 ? 1 : target, lo, hi, &s.u.select, each).cut;
+      cut = true;
+    }
+    if (cut) keep.upto(lo, places);
+  }
+  uint64_t by_vec[NV], total = 0;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const Held<T> h = raw[v].fresh();
+    by_vec[v] = 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) by_vec[v] += keep.mass(h[e], (v * 64 + lane) * V + e);
+    total += by_vec[v];
+  }
+  total = wave_sum_int(total);
+  uint64_t t = floor_part(total, uniform(a, row)), step = 0;
+  bool found = false;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if (found) continue;
+    step = NV == 1 ? total : wave_sum_int(by_vec[v]);
+    if (t >= step) {
+      t -= step;
+      continue;
+    }
+    found = true;
+    const uint64_t upto = wave_scan(by_vec[v], lane);
+    uint64_t before = upto - by_vec[v];
+    const Held<T> h = raw[v].fresh();
+    if (t >= before && t < upto) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const uint64_t w = keep.mass(h[e], (v * 64 + lane) * V + e);
+        if (t >= before && t < before + w)
+          write_one(a, row, (v * 64 + lane) * V + e, (float)((double)w / (double)total));
+        before += w;
+      }
+    }
+  }
+}
+
+// ---- long rows with a short top-k -----------------------------------------------------------------
+struct ListLds {
+  BlockTopLds top;
+  uint64_t w[BLOCK_TOP];
+  int c[BLOCK_TOP];
+};
+
+__device__ __forceinline__ bool short_list(const Settings& set) { return set.top_k > 0 && set.top_k <= BLOCK_TOP; }
+
+__device__ __forceinline__ void draw_or_none(const SampleCall& a, int64_t row, Settings set, Places places, int n,
+                                             ListLds* s) {
+  if (threadIdx.x >= 64) return;
+  if (n == 0) {
+    if (threadIdx.x == 0) write_one(a, row, -1, 0.f);
+  } else if (!(set.T > 0.f)) {
+    if (threadIdx.x == 0) write_one(a, row, places.cls(s->top.sorted[0]), 1.f);
+  } else {
+    draw_from_list<BLOCK_TOP>(a, row, set, places, s->top.sorted, n, threadIdx.x, s->w, s->c);
+  }
+}
+
+// rows whose top-k is not short are left to another kernel
+template <class T>
+__global__ __launch_bounds__(TOP_THREADS) void sample_list_kernel(SampleCall a) {
+  __shared__ ListLds s;
+  const int64_t row = blockIdx.x;
+  const Settings set = settings(a, row);
+  if (!short_list(set)) return;
+  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
+  const Places places(a.K);
+  const int n = block_top<T>(z, 0, a.K, places, set.top_k, &s.top);
+  draw_or_none(a, row, set, places, n, &s);
+}
+
+// lists[row][part][k], k the same for all rows
+template <class T>
+__global__ __launch_bounds__(TOP_THREADS) void sample_parts_kernel(SampleCall a, int len, uint64_t* lists) {
+  __shared__ BlockTopLds s;
+  const int64_t row = blockIdx.y;
+  const int k = a.top_k_all, c0 = blockIdx.x * len;
+  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
+  const int n = block_top<T>(z, c0, min(a.K, c0 + len), Places(a.K), k, &s);
+  uint64_t* out = lists + (row * gridDim.x + blockIdx.x) * k;
+  for (int r = threadIdx.x; r < k; r += TOP_THREADS) out[r] = r < n ? s.sorted[r] : 0;
+}
+__global__ __launch_bounds__(TOP_THREADS) void sample_merge_kernel(SampleCall a, int parts, const uint64_t* lists) {
+  __shared__ ListLds s;
+  const int64_t row = blockIdx.x;
+  const int k = a.top_k_all;
+  const Places places(a.K);
+  const int n = merge_top(lists + row * parts * k, parts * k, places, k, &s.top);
+  draw_or_none(a, row, settings(a, row), places, n, &s);
+}
+
+// ---- one block, row in registers ------------------------------------------------------------------
+constexpr int MASS_BINS = 1024;
+constexpr int MASS_LIST = 1024;
+template <int NT, int NV>
+struct RowLds {
+  union {
+    struct {
+      uint64_t mass[MASS_BINS];
+      uint64_t place[MASS_LIST], w[MASS_LIST];
+    } h;
+    SelectLds<SELECT_BINS> select;
+  } u;
+  uint64_t scratch[NT / 64];
+  uint64_t by_wave[NV * (NT / 64)];
+  uint64_t out[3];
+  int n;
+};
+
+// SKIP: rows with a short top-k have been drawn already
+template <class T, int NT, int NV, bool SKIP>
+__global__ __launch_bounds__(NT) void sample_row_kernel(SampleCall a) {
+  constexpr int V = Vec<T>::N, WAVES = NT / 64;
+  __shared__ RowLds<NT, NV> s;
+  const int64_t row = blockIdx.x;
+  const Settings set = settings(a, row);
+  if (SKIP && short_list(set)) return;
+  const int K = a.K, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
+  const Places places(K);
+  auto add = [](uint64_t x, uint64_t y) { return x + y; };
+  Held<T> raw[NV];
+  load_row<T, NT, NV>(raw, z, tid, K);
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < V; ++e) m = fmaxf(m, raw[v][e]);
+  // one pass over the row: f(logit, class)
+  auto pass = [&](auto f) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const Held<T> h = raw[v].fresh();
+#pragma unroll
+      for (int e = 0; e < V; ++e) f(h[e], (v * NT + tid) * V + e);
+    }
+  };
+  m = block_reduce<NT>(m, reinterpret_cast<float*>(s.scratch), [](float x, float y) { return fmaxf(x, y); });
+  if (m == -__builtin_inff() || !(set.T > 0.f)) {
+    int first = K;
+    pass([&](float x, int i) { first = x == m ? min(first, i) : first; });
+    first = block_reduce<NT>(first, reinterpret_cast<int*>(s.scratch), [](int x, int y) { return min(x, y); });
+    const bool none = m == -__builtin_inff();
+    if (tid == 0) write_one(a, row, none ? -1 : first, none ? 0.f : 1.f);
+    return;
+  }
+  Keep keep = keep_all(m, set);
+  auto each = [&](auto f) {
+    pass([&](float x, int i) {
+      const uint32_t key = order_key(x);
+      if (key > KEY_MASKED) f(places.of(key, i), weight(x, m, keep.c));
+    });
+  };
+  uint64_t lo = places.last(KEY_MASKED + 1);
+  const uint64_t hi = places.first(order_key(m)) - 1;
+  if (set.top_k > 0 && set.top_k < K) {
+    int valid = 0;
+    pass([&](float x, int) { valid += x > -__builtin_inff() ? 1 : 0; });
+    valid = block_reduce<NT>(valid, reinterpret_cast<int*>(s.scratch), [](int x, int y) { return x + y; });
+    if (set.top_k < valid) {
+      lo = select_prefix<NT, SELECT_BINS>(false, set.top_k, lo, hi, &s.u.select, each).cut;
+      keep.upto(lo, places);
+      __syncthreads();
+    }
+  }
+  if (set.top_p < 1.f) {
+    // masses by bins of equal width in z, the largest logit in bin 0; past 30 T a weight is nothing
+    for (int b = tid; b < MASS_BINS; b += NT) s.u.h.mass[b] = 0;
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    const float scale = (float)(MASS_BINS / 30.0) / set.T;
+    auto bin = [&](float x) { return (int)fminf(fmaxf((m - x) * scale, 0.f), (float)(MASS_BINS - 1)); };
+    const Keep first{m, keep.c, keep.z, keep.cls, 0};
+    pass([&](float x, int i) {
+      const uint64_t w = first.mass(x, i);
+      if (w != 0) atomicAdd((unsigned long long*)&s.u.h.mass[bin(x)], (unsigned long long)w);
+    });
+    __syncthreads();
+    if (tid < 64) {
+      constexpr int PER = MASS_BINS / 64;
+      uint64_t own = 0;
+      for (int b = 0; b < PER; ++b) own += s.u.h.mass[tid * PER + b];
+      const uint64_t upto = wave_scan(own, tid), target = max(ceil_part(lane_value(upto, 63), fmaxf(set.top_p, 0.f)), (uint64_t)1);
+      uint64_t before = upto - own;
+      if (before < target && upto >= target) {
+        int b = tid * PER;
+        while (before + s.u.h.mass[b] < target) before += s.u.h.mass[b++];
+        s.out[0] = b, s.out[1] = before, s.out[2] = target;
+      }
+    }
+    __syncthreads();
+    const int at = (int)s.out[0];
+    const uint64_t above = s.out[1], target = s.out[2];
+    pass([&](float x, int i) {
+      if (x > -__builtin_inff() && bin(x) == at) {
+        const uint64_t w = first.mass(x, i);
+        if (w != 0) {
+          const int j = atomicAdd(&s.n, 1);
+          if (j < MASS_LIST) s.u.h.place[j] = places.of(order_key(x), i), s.u.h.w[j] = w;
+        }
+      }
+    });
+    __syncthreads();
+    const int n = s.n;
+    if (n <= MASS_LIST) {
+      for (int j = tid; j < n; j += NT) {
+        const uint64_t mine = s.u.h.place[j], w = s.u.h.w[j];
+        uint64_t before = above;
+        for (int i = 0; i < n; ++i) before += s.u.h.place[i] > mine ? s.u.h.w[i] : 0;
+        if (before < target && before + w >= target) s.out[0] = mine;
+      }
+      __syncthreads();
+      lo = s.out[0];
+    } else {  // many classes next to the border: equal logits, or a wide bin
+      lo = select_prefix<NT, SELECT_BINS>(true, target, lo, hi, &s.u.select, each).cut;
+    }
+    keep.upto(lo, places);
+  }
+  // kept mass of every wave's vector v, in class order
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    uint64_t w = 0;
+    if (v * NT * V < K) {
+      const Held<T> h = raw[v].fresh();
+#pragma unroll
+      for (int e = 0; e < V; ++e) w += keep.mass(h[e], (v * NT + tid) * V + e);
+      w = wave_sum_int(w);
+    }
+    if (lane == 0) s.by_wave[v * WAVES + wave] = w;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    constexpr int PER = (NV * WAVES + 63) / 64;
+    uint64_t own = 0;
+    for (int i = 0; i < PER; ++i)
+      if (tid * PER + i < NV * WAVES) own += s.by_wave[tid * PER + i];
+    const uint64_t upto = wave_scan(own, tid), total = lane_value(upto, 63), t = floor_part(total, uniform(a, row));
+    uint64_t before = upto - own;
+    if (t >= before && t < upto) {
+      int i = tid * PER;
+      while (t >= before + s.by_wave[i]) before += s.by_wave[i++];
+      s.out[0] = i, s.out[1] = t - before, s.out[2] = total;
+    }
+  }
+  __syncthreads();
+  const int pick = (int)s.out[0];
+  if (wave != pick % WAVES) return;
+  const uint64_t t = s.out[1], total = s.out[2];
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+    if (v == pick / WAVES) {
+      const Held<T> h = raw[v].fresh();
+      uint64_t own[V], sum = 0;
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum += own[e] = keep.mass(h[e], (v * NT + tid) * V + e);
+      uint64_t before = wave_scan(sum, lane) - sum;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (t >= before && t < before + own[e])
+          write_one(a, row, (v * NT + tid) * V + e, (float)((double)own[e] / (double)total));
+        before += own[e];
+      }
+    }
+}
+
+// ---- one block, row in memory ---------------------------------------------------------------------
+// SKIP as above
+template <class T, int NT, bool SKIP>
+__global__ __launch_bounds__(NT) void sample_long_kernel(SampleCall a) {
+  constexpr int V = Vec<T>::N, STEP = NT * V, MAX_STEPS = LOGIT_MAX_CLASSES / STEP;
+  __shared__ SelectLds<SELECT_BINS> sel;
   __shared__ uint64_t scratch[NT / 64];
   __shared__ uint64_t step_mass[MAX_STEPS];
   __shared__ uint64_t pick[2];
@@ -61,6 +489,7 @@ __global__ __launch_bounds__(NT) void sample_block_kernel(SampleCall a) {
   const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
   const Places places(K);
   const Settings set = settings(a, row);
+  if (SKIP && short_list(set)) return;
   auto add = [](uint64_t x, uint64_t y) { return x + y; };
   uint64_t best = 0;  // largest place
   uint32_t lo = 0xffffffffu, n = 0;
@@ -99,7 +528,7 @@ __global__ __launch_bounds__(NT) void sample_block_kernel(SampleCall a) {
   };
   uint64_t cut = 0, mass = 0;
   if (set.top_k > 0 && (uint64_t)set.top_k < valid) {
-    const Prefix p = select_prefix<NT>(false, (uint64_t)set.top_k, places.last(lo), best, &sel, each);
+    const Prefix p = select_prefix<NT, SELECT_BINS>(false, (uint64_t)set.top_k, places.last(lo), best, &sel, each);
     cut = p.cut, mass = p.mass;
   } else if (set.top_p < 1.f) {
     each([&](uint64_t, uint64_t w) { mass += w; });
@@ -109,7 +538,7 @@ __global__ __launch_bounds__(NT) void sample_block_kernel(SampleCall a) {
     uint64_t target = ceil_part(mass, fmaxf(set.top_p, 0.f));
     if (target == 0) target = 1;
     const uint64_t from = cut > places.last(lo) ? cut : places.last(lo);
-    cut = select_prefix<NT>(true, target, from, best, &sel, each).cut;
+    cut = select_prefix<NT, SELECT_BINS>(true, target, from, best, &sel, each).cut;
   }
   const uint64_t least = least_weight(set.min_p);
   // kept mass of every step of NT vectors, in class order
@@ -167,21 +596,99 @@ __global__ __launch_bounds__(NT) void sample_block_kernel(SampleCall a) {
   }
 }
 
+struct Plan {
+  int parts = 1, len = 0;
+};
+
+// As top_logits cuts rows, where one short k holds for all of them.
+template <class T>
+Plan make_plan(const SampleCall& a) {
+  Plan p;
+  p.len = a.K;
+  if (a.top_k != nullptr || a.top_k_all < 1 || a.top_k_all > BLOCK_TOP) return p;
+  constexpr int STEP = TOP_THREADS * Vec<T>::N;
+  const int steps = (a.K + STEP - 1) / STEP;
+  const int64_t want = std::min<int64_t>({(512 + a.B - 1) / a.B, steps / 8, MERGE_PLACES / a.top_k_all, 64});
+  p.parts = (int)std::max<int64_t>(1, want);
+  p.len = (steps + p.parts - 1) / p.parts * STEP;
+  p.parts = (a.K + p.len - 1) / p.len;
+  return p;
+}
+
+template <class T>
+bool fits_wave(int K) {
+  return K <= 2048;
+}
+
+template <class T, int NV>
+void launch_wave(const SampleCall& a, hipStream_t stream) {
+  const dim3 grid((unsigned)((a.B + 3) / 4));
+  const bool all = a.top_k == nullptr && a.top_k_all == 0 && a.top_p == nullptr && a.top_p_all >= 1.f;
+  if (all)
+    hipLaunchKernelGGL((sample_wave_kernel<T, NV, true>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((sample_wave_kernel<T, NV, false>), grid, dim3(256), 0, stream, a);
+}
+
+template <class T, bool SKIP, int NT, int NV>
+void launch_row(const SampleCall& a, hipStream_t stream) {
+  hipLaunchKernelGGL((sample_row_kernel<T, NT, NV, SKIP>), dim3((unsigned)a.B), dim3(NT), 0, stream, a);
+}
+
+template <class T, bool SKIP>
+void launch_long(const SampleCall& a, hipStream_t stream) {
+  const int vecs = (a.K + Vec<T>::N - 1) / Vec<T>::N;
+  if (vecs <= 256 * 4) return launch_row<T, SKIP, 256, 4>(a, stream);
+  if (vecs <= 512 * 4) return launch_row<T, SKIP, 512, 4>(a, stream);
+  if (vecs <= 1024 * 4) return launch_row<T, SKIP, 1024, 4>(a, stream);
+  if (vecs <= 1024 * 8) return launch_row<T, SKIP, 1024, 8>(a, stream);
+  if (vecs <= 1024 * 16) return launch_row<T, SKIP, 1024, 16>(a, stream);
+  hipLaunchKernelGGL((sample_long_kernel<T, 1024, SKIP>), dim3((unsigned)a.B), dim3(1024), 0, stream, a);
+}
+
 template <class T>
 void run_sample(const SampleCall& a, hipStream_t stream) {
-  if (a.K <= 8 * 256 * Vec<T>::N) {
-    hipLaunchKernelGGL((sample_block_kernel<T, 256>), dim3((unsigned)a.B), dim3(256), 0, stream, a);
+  if (fits_wave<T>(a.K)) {
+    const int vecs = (a.K + Vec<T>::N - 1) / Vec<T>::N;
+    if (vecs <= 64)
+      launch_wave<T, 1>(a, stream);
+    else if (vecs <= 128)
+      launch_wave<T, 2>(a, stream);
+    else if (vecs <= 256)
+      launch_wave<T, 4>(a, stream);
+    else if constexpr (sizeof(T) == 4)
+      launch_wave<T, 8>(a, stream);
+  } else if (a.top_k != nullptr) {  // each row its own k: the short ones first, the others after
+    hipLaunchKernelGGL((sample_list_kernel<T>), dim3((unsigned)a.B), dim3(TOP_THREADS), 0, stream, a);
+    launch_long<T, true>(a, stream);
+  } else if (a.top_k_all >= 1 && a.top_k_all <= BLOCK_TOP) {
+    const Plan p = make_plan<T>(a);
+    if (p.parts == 1) {
+      hipLaunchKernelGGL((sample_list_kernel<T>), dim3((unsigned)a.B), dim3(TOP_THREADS), 0, stream, a);
+    } else {
+      uint64_t* lists = static_cast<uint64_t*>(a.workspace);
+      hipLaunchKernelGGL((sample_parts_kernel<T>), dim3((unsigned)p.parts, (unsigned)a.B), dim3(TOP_THREADS), 0, stream,
+                         a, p.len, lists);
+      hipLaunchKernelGGL(sample_merge_kernel, dim3((unsigned)a.B), dim3(TOP_THREADS), 0, stream, a, p.parts, lists);
+    }
   } else {
-    hipLaunchKernelGGL((sample_block_kernel<T, 1024>), dim3((unsigned)a.B), dim3(1024), 0, stream, a);
+    launch_long<T, false>(a, stream);
   }
   MLAPI_HIP_CHECK(hipGetLastError());
 }
 
+template <class T>
+size_t list_bytes(const SampleCall& a) {
+  if (fits_wave<T>(a.K)) return 0;
+  const Plan p = make_plan<T>(a);
+  return p.parts == 1 ? 0 : (size_t)a.B * p.parts * a.top_k_all * sizeof(uint64_t);
+}
+
 }  // namespace
 
-size_t sample_workspace(const SampleCall& call) {
-  (void)call;
-  return 0;
+size_t sample_workspace(const SampleCall& c) {
+  if (c.B <= 0 || c.K < 1) return 0;
+  return c.dt == DT_F32 ? list_bytes<float>(c) : list_bytes<__bf16>(c);
 }
 
 void launch_sample(const SampleCall& c, hipStream_t stream) {
@@ -189,6 +696,7 @@ void launch_sample(const SampleCall& c, hipStream_t stream) {
   if (c.K < 1 || c.K > LOGIT_MAX_CLASSES) throw std::invalid_argument("sample: 1 <= K <= 2^20 classes");
   if (c.ldz < c.K) throw std::invalid_argument("sample: row stride below K");
   if (c.B > 0x7fffffff) throw std::invalid_argument("sample: more than 2^31 rows");
+  if (c.ws_bytes < sample_workspace(c)) throw std::invalid_argument("sample: workspace too small");
   if (c.dt == DT_F32) return run_sample<float>(c, stream);
   if (c.dt == DT_BF16) return run_sample<__bf16>(c, stream);
   if (c.dt == DT_F16) return run_sample<_Float16>(c, stream);

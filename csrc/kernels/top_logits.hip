@@ -84,7 +84,7 @@ __global__ __launch_bounds__(TOP_THREADS) void top_merge_kernel(TopArgs a, int p
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void top_select_kernel(TopArgs a) {
   constexpr int V = Vec<T>::N;
-  __shared__ SelectLds sel;
+  __shared__ SelectLds<SELECT_BINS> sel;
   __shared__ uint64_t list[LOGIT_MAX_TOP];
   __shared__ uint32_t scratch[NT / 64];
   __shared__ int found;
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(NT) void top_select_kernel(TopArgs a) {
       }
     }
   };
-  const Prefix p = select_prefix<NT>(false, take, places.last(lo), places.first(hi) - 1, &sel, each);
+  const Prefix p = select_prefix<NT, SELECT_BINS>(false, take, places.last(lo), places.first(hi) - 1, &sel, each);
   if (threadIdx.x == 0) found = 0;
   __syncthreads();
   each([&](uint64_t place, uint64_t) {
