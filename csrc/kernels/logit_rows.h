@@ -195,9 +195,11 @@ __device__ __forceinline__ float key_logit(uint32_t key) {
 // be off by: the exponential is evaluated in f64 (an f32 one, 2^-24 off, would move a border of 65536
 // rows of 1000 classes often enough to be seen).
 constexpr int WEIGHT_BITS = 42;
+// z may be -inf (weight 0) but not NaN.
 __device__ __forceinline__ uint64_t weight(float z, float m, double c /* log2(e) / T */) {
-  // -inf, NaN and all that rounds to nothing end at 2^-16
-  const double y = __builtin_fmax(__builtin_fma((double)z - (double)m, c, (double)WEIGHT_BITS), -16.0);
+  // from above: inf - inf, a NaN, where m is inf; from below: all that rounds to nothing
+  const double x = __builtin_fma((double)z - (double)m, c, (double)WEIGHT_BITS);
+  const double y = __builtin_fmax(__builtin_fmin(x, (double)WEIGHT_BITS), -16.0);
   const double n = __builtin_rint(y), f = y - n;
   // 2^f on [-1/2, 1/2]: 1 + f q(f), q of degree 8 through (2^f - 1) / f at nine Chebyshev points,
   // 2^-44.6 off; exactly 1 at f = 0, so equal logits weigh the same
@@ -213,9 +215,9 @@ __device__ __forceinline__ uint64_t weight(float z, float m, double c /* log2(e)
   p = __builtin_fma(p, f, 1.0);
   // the integer nearest to p 2^n falls out of the low bits of a sum with 2^52
   const double w = __builtin_ldexp(p, (int)n) + 0x1p52;
-  const uint64_t k = __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
-  return z == m ? 1ull << WEIGHT_BITS : k;  // also for m = inf, which has no difference to itself
+  return __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
 }
+__device__ __forceinline__ float no_nan(float z) { return fmaxf(z, -__builtin_inff()); }
 
 // floor(u mass) and ceil(p mass) for a fraction 0 <= u, p < 1, exactly
 __device__ __forceinline__ uint64_t fraction_bits(float u) { return (uint64_t)((double)u * 0x1p64); }

@@ -17,8 +17,7 @@
 // Which kernel draws a row:
 //   rows of up to 2048 classes: one wave, from registers (sample_wave_kernel);
 //   longer rows with a short top-k: the k first classes by one pass (row_top.h), few long rows in parts;
-//   longer rows else: one block, from registers, two passes of weights (sample_row_kernel);
-//   rows that registers do not hold: one block, from memory (sample_long_kernel).
+//   longer rows else: one block, from memory, two passes of weights (sample_row_kernel).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -62,8 +61,11 @@ struct Keep {
   float z;  // the last class kept: its logit and its number
   int cls;
   uint64_t least;
+  // every class is kept
+  __device__ __forceinline__ bool all() const { return z == -__builtin_inff() && least == 0; }
+  __device__ __forceinline__ uint64_t any_mass(float x) const { return weight(no_nan(x), m, c); }
   __device__ __forceinline__ uint64_t mass(float x, int i) const {
-    const uint64_t w = weight(x, m, c);
+    const uint64_t w = any_mass(x);
     return (x > z || (x == z && i <= cls)) && w >= least ? w : 0;
   }
   __device__ __forceinline__ void upto(uint64_t place, Places places) {
@@ -211,13 +213,19 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleCall a) {
     }
     if (cut) keep.upto(lo, places);
   }
+  const bool all = keep.all();
   uint64_t by_vec[NV], total = 0;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const Held<T> h = raw[v].fresh();
     by_vec[v] = 0;
+    if (all) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) by_vec[v] += keep.mass(h[e], (v * 64 + lane) * V + e);
+      for (int e = 0; e < V; ++e) by_vec[v] += keep.any_mass(h[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) by_vec[v] += keep.mass(h[e], (v * 64 + lane) * V + e);
+    }
     total += by_vec[v];
   }
   total = wave_sum_int(total);
@@ -301,56 +309,100 @@ __global__ __launch_bounds__(TOP_THREADS) void sample_merge_kernel(SampleCall a,
   draw_or_none(a, row, settings(a, row), places, n, &s);
 }
 
-// ---- one block, row in registers ------------------------------------------------------------------
-constexpr int MASS_BINS = 1024;
+// ---- one block, row in memory ---------------------------------------------------------------------
+// A row is read four times: for its maximum, the masses by logit, the classes next to the border, the
+// masses by class. The reads after the first come from the caches and cost little beside the weights:
+// 256 rows of 65536 bf16 took 68 us with the row in registers, whose unrolled passes outgrow the
+// instruction cache.
 constexpr int MASS_LIST = 1024;
-template <int NT, int NV>
+template <int NT>
 struct RowLds {
+  // twice the threads: 65536 normal logits leave about 150 classes in the bin of a border
+  static constexpr int BINS = NT < 512 ? 1024 : 2 * NT;
+  static constexpr int SEGMENTS = NT < 512 ? 1024 : LOGIT_MAX_CLASSES / 256;  // a wave's vectors of one step
   union {
     struct {
-      uint64_t mass[MASS_BINS];
+      uint64_t mass[BINS];
       uint64_t place[MASS_LIST], w[MASS_LIST];
     } h;
+    uint64_t segment[SEGMENTS];
     SelectLds<SELECT_BINS> select;
   } u;
   uint64_t scratch[NT / 64];
-  uint64_t by_wave[NV * (NT / 64)];
   uint64_t out[3];
   int n;
 };
+constexpr int SMALL_BLOCK_CLASSES = 8192;  // longest rows of 256 threads: 32 segments
+
+// Where the running sum of x[0 .. NT PER) (PER to a thread, in order) passes `target(sum of all)`: out = index,
+// sum before it, target. The sum of all reaches the target.
+template <int NT, int PER, class Target>
+__device__ __forceinline__ void crossing(const uint64_t* x, int count, uint64_t* scratch, uint64_t* out,
+                                         Target&& target) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint64_t own = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (tid * PER + i < count) own += x[tid * PER + i];
+  uint64_t upto = wave_scan(own, lane), all = 0;
+  __syncthreads();
+  if (lane == 63) scratch[wave] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    if (w < wave) upto += scratch[w];
+    all += scratch[w];
+  }
+  const uint64_t t = target(all);
+  uint64_t before = upto - own;
+  if (before < t && upto >= t) {
+    int i = tid * PER;
+    while (before + x[i] < t) before += x[i++];
+    out[0] = i, out[1] = before, out[2] = t;
+  }
+  __syncthreads();
+}
 
 // SKIP: rows with a short top-k have been drawn already
-template <class T, int NT, int NV, bool SKIP>
+template <class T, int NT, bool SKIP>
 __global__ __launch_bounds__(NT) void sample_row_kernel(SampleCall a) {
-  constexpr int V = Vec<T>::N, WAVES = NT / 64;
-  __shared__ RowLds<NT, NV> s;
+  constexpr int V = Vec<T>::N, STEP = NT * V, WAVES = NT / 64, U = 2;
+  typedef RowLds<NT> Lds;
+  __shared__ Lds s;
   const int64_t row = blockIdx.x;
   const Settings set = settings(a, row);
   if (SKIP && short_list(set)) return;
   const int K = a.K, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
   const Places places(K);
-  auto add = [](uint64_t x, uint64_t y) { return x + y; };
-  Held<T> raw[NV];
-  load_row<T, NT, NV>(raw, z, tid, K);
-  float m = -__builtin_inff();
+  // one pass over the row: f(vector, its first class), for every thread the same number of times
+  auto vectors = [&](auto f) {
+    int base = 0;
+    for (; base + U * STEP <= K; base += U * STEP) {
+      Held<T> h[U];
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+      for (int u = 0; u < U; ++u) h[u].load(z, base + u * STEP + tid * V);
 #pragma unroll
-    for (int e = 0; e < V; ++e) m = fmaxf(m, raw[v][e]);
-  // one pass over the row: f(logit, class)
-  auto pass = [&](auto f) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const Held<T> h = raw[v].fresh();
-#pragma unroll
-      for (int e = 0; e < V; ++e) f(h[e], (v * NT + tid) * V + e);
+      for (int u = 0; u < U; ++u) f(h[u], base + u * STEP + tid * V);
+    }
+    for (; base < K; base += STEP) {
+      Held<T> h;
+      h.load(z, base + tid * V, K);
+      f(h, base + tid * V);
     }
   };
+  auto pass = [&](auto f) {
+    vectors([&](const Held<T>& h, int i) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f(h[e], i + e);
+    });
+  };
+  float m = -__builtin_inff();
+  pass([&](float x, int) { m = fmaxf(m, x); });
   m = block_reduce<NT>(m, reinterpret_cast<float*>(s.scratch), [](float x, float y) { return fmaxf(x, y); });
   if (m == -__builtin_inff() || !(set.T > 0.f)) {
     int first = K;
-    pass([&](float x, int i) { first = x == m ? min(first, i) : first; });
+    pass([&](float x, int i) { first = x == m && i < K ? min(first, i) : first; });
     first = block_reduce<NT>(first, reinterpret_cast<int*>(s.scratch), [](int x, int y) { return min(x, y); });
     const bool none = m == -__builtin_inff();
     if (tid == 0) write_one(a, row, none ? -1 : first, none ? 0.f : 1.f);
@@ -377,34 +429,29 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleCall a) {
   }
   if (set.top_p < 1.f) {
     // masses by bins of equal width in z, the largest logit in bin 0; past 30 T a weight is nothing
-    for (int b = tid; b < MASS_BINS; b += NT) s.u.h.mass[b] = 0;
+    for (int b = tid; b < Lds::BINS; b += NT) s.u.h.mass[b] = 0;
     if (tid == 0) s.n = 0;
     __syncthreads();
-    const float scale = (float)(MASS_BINS / 30.0) / set.T;
-    auto bin = [&](float x) { return (int)fminf(fmaxf((m - x) * scale, 0.f), (float)(MASS_BINS - 1)); };
+    const float scale = (float)(Lds::BINS / 30.0) / set.T;
+    auto depth = [&](float x) { return fminf(fmaxf((m - x) * scale, 0.f), (float)(Lds::BINS - 1)); };
     const Keep first{m, keep.c, keep.z, keep.cls, 0};
-    pass([&](float x, int i) {
-      const uint64_t w = first.mass(x, i);
-      if (w != 0) atomicAdd((unsigned long long*)&s.u.h.mass[bin(x)], (unsigned long long)w);
+    auto count = [&](float x, uint64_t w) {
+      if (w != 0) atomicAdd((unsigned long long*)&s.u.h.mass[(int)depth(x)], (unsigned long long)w);
+    };
+    if (first.all())
+      pass([&](float x, int) { count(x, first.any_mass(x)); });
+    else
+      pass([&](float x, int i) { count(x, first.mass(x, i)); });
+    __syncthreads();
+    crossing<NT, Lds::BINS / NT>(s.u.h.mass, Lds::BINS, s.scratch, s.out, [&](uint64_t mass) {
+      const uint64_t t = ceil_part(mass, fmaxf(set.top_p, 0.f));
+      return t == 0 ? 1 : t;
     });
-    __syncthreads();
-    if (tid < 64) {
-      constexpr int PER = MASS_BINS / 64;
-      uint64_t own = 0;
-      for (int b = 0; b < PER; ++b) own += s.u.h.mass[tid * PER + b];
-      const uint64_t upto = wave_scan(own, tid), target = max(ceil_part(lane_value(upto, 63), fmaxf(set.top_p, 0.f)), (uint64_t)1);
-      uint64_t before = upto - own;
-      if (before < target && upto >= target) {
-        int b = tid * PER;
-        while (before + s.u.h.mass[b] < target) before += s.u.h.mass[b++];
-        s.out[0] = b, s.out[1] = before, s.out[2] = target;
-      }
-    }
-    __syncthreads();
-    const int at = (int)s.out[0];
     const uint64_t above = s.out[1], target = s.out[2];
+    const float near = (float)(int)s.out[0];
     pass([&](float x, int i) {
-      if (x > -__builtin_inff() && bin(x) == at) {
+      const float d = depth(x);
+      if (d >= near && d < near + 1.f) {
         const uint64_t w = first.mass(x, i);
         if (w != 0) {
           const int j = atomicAdd(&s.n, 1);
@@ -427,172 +474,43 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleCall a) {
       lo = select_prefix<NT, SELECT_BINS>(true, target, lo, hi, &s.u.select, each).cut;
     }
     keep.upto(lo, places);
+    __syncthreads();
   }
-  // kept mass of every wave's vector v, in class order
+  // kept mass of every wave's vectors of one step, in class order
+  auto segments = [&](auto mass) {
+    vectors([&](const Held<T>& h, int i) {
+      uint64_t w = 0;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    uint64_t w = 0;
-    if (v * NT * V < K) {
-      const Held<T> h = raw[v].fresh();
-#pragma unroll
-      for (int e = 0; e < V; ++e) w += keep.mass(h[e], (v * NT + tid) * V + e);
+      for (int e = 0; e < V; ++e) w += mass(h[e], i + e);
       w = wave_sum_int(w);
-    }
-    if (lane == 0) s.by_wave[v * WAVES + wave] = w;
-  }
-  __syncthreads();
-  if (tid < 64) {
-    constexpr int PER = (NV * WAVES + 63) / 64;
-    uint64_t own = 0;
-    for (int i = 0; i < PER; ++i)
-      if (tid * PER + i < NV * WAVES) own += s.by_wave[tid * PER + i];
-    const uint64_t upto = wave_scan(own, tid), total = lane_value(upto, 63), t = floor_part(total, uniform(a, row));
-    uint64_t before = upto - own;
-    if (t >= before && t < upto) {
-      int i = tid * PER;
-      while (t >= before + s.by_wave[i]) before += s.by_wave[i++];
-      s.out[0] = i, s.out[1] = t - before, s.out[2] = total;
-    }
-  }
-  __syncthreads();
-  const int pick = (int)s.out[0];
-  if (wave != pick % WAVES) return;
-  const uint64_t t = s.out[1], total = s.out[2];
-#pragma unroll
-  for (int v = 0; v < NV; ++v)
-    if (v == pick / WAVES) {
-      const Held<T> h = raw[v].fresh();
-      uint64_t own[V], sum = 0;
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum += own[e] = keep.mass(h[e], (v * NT + tid) * V + e);
-      uint64_t before = wave_scan(sum, lane) - sum;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (t >= before && t < before + own[e])
-          write_one(a, row, (v * NT + tid) * V + e, (float)((double)own[e] / (double)total));
-        before += own[e];
-      }
-    }
-}
-
-// ---- one block, row in memory ---------------------------------------------------------------------
-// SKIP as above
-template <class T, int NT, bool SKIP>
-__global__ __launch_bounds__(NT) void sample_long_kernel(SampleCall a) {
-  constexpr int V = Vec<T>::N, STEP = NT * V, MAX_STEPS = LOGIT_MAX_CLASSES / STEP;
-  __shared__ SelectLds<SELECT_BINS> sel;
-  __shared__ uint64_t scratch[NT / 64];
-  __shared__ uint64_t step_mass[MAX_STEPS];
-  __shared__ uint64_t pick[2];
-  const int64_t row = blockIdx.x;
-  const int K = a.K;
-  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
-  const Places places(K);
-  const Settings set = settings(a, row);
-  if (SKIP && short_list(set)) return;
-  auto add = [](uint64_t x, uint64_t y) { return x + y; };
-  uint64_t best = 0;  // largest place
-  uint32_t lo = 0xffffffffu, n = 0;
-  for (int i = (int)threadIdx.x * V; i < K; i += STEP) {
-    const typename Vec<T>::type raw = load_vec(z, i, K);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const uint32_t key = order_key((float)raw[e]);
-      if (key > KEY_MASKED) {
-        const uint64_t place = places.of(key, i + e);
-        best = best > place ? best : place;
-        lo = min(lo, key);
-        ++n;
-      }
-    }
-  }
-  best = block_reduce<NT>(best, scratch, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
-  lo = (uint32_t)block_reduce<NT>((uint64_t)lo, scratch, [](uint64_t x, uint64_t y) { return x < y ? x : y; });
-  const uint64_t valid = block_reduce<NT>((uint64_t)n, scratch, add);
-  if (valid == 0 || !(set.T > 0.f)) {
-    if (threadIdx.x == 0) a.idx[row] = valid == 0 ? -1 : places.cls(best), a.prob[row] = valid == 0 ? 0.f : 1.f;
-    return;
-  }
-  const float m = key_logit((uint32_t)(best >> places.ib));
-  const double c = 1.4426950408889634074 / (double)set.T;
-  auto each = [&](auto f) {
-    for (int i = (int)threadIdx.x * V; i < K; i += STEP) {
-      const typename Vec<T>::type raw = load_vec(z, i, K);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float x = (float)raw[e];
-        const uint32_t key = order_key(x);
-        if (key > KEY_MASKED) f(places.of(key, i + e), weight(x, m, c));
-      }
-    }
+      if (lane == 0) s.u.segment[i / (64 * V)] = w;
+    });
   };
-  uint64_t cut = 0, mass = 0;
-  if (set.top_k > 0 && (uint64_t)set.top_k < valid) {
-    const Prefix p = select_prefix<NT, SELECT_BINS>(false, (uint64_t)set.top_k, places.last(lo), best, &sel, each);
-    cut = p.cut, mass = p.mass;
-  } else if (set.top_p < 1.f) {
-    each([&](uint64_t, uint64_t w) { mass += w; });
-    mass = block_reduce<NT>(mass, scratch, add);
-  }
-  if (set.top_p < 1.f) {
-    uint64_t target = ceil_part(mass, fmaxf(set.top_p, 0.f));
-    if (target == 0) target = 1;
-    const uint64_t from = cut > places.last(lo) ? cut : places.last(lo);
-    cut = select_prefix<NT, SELECT_BINS>(true, target, from, best, &sel, each).cut;
-  }
-  const uint64_t least = least_weight(set.min_p);
-  // kept mass of every step of NT vectors, in class order
-  const int steps = (K + STEP - 1) / STEP;
-  for (int s = threadIdx.x; s < steps; s += NT) step_mass[s] = 0;
-  __syncthreads();
-  auto vec_mass = [&](int i) {
-    uint64_t v = 0;
-    if (i < K) {
-      const typename Vec<T>::type raw = load_vec(z, i, K);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float x = (float)raw[e];
-        const uint32_t key = order_key(x);
-        if (key > KEY_MASKED && places.of(key, i + e) >= cut) {
-          const uint64_t w = weight(x, m, c);
-          if (w >= least) v += w;
-        }
-      }
-    }
-    return v;
-  };
-  for (int s = 0; s < steps; ++s) {
-    const uint64_t v = wave_sum_int(vec_mass(s * STEP + (int)threadIdx.x * V));
-    if ((threadIdx.x & 63) == 0) atomicAdd((unsigned long long*)&step_mass[s], (unsigned long long)v);
-  }
+  if (keep.all())
+    segments([&](float x, int) { return keep.any_mass(x); });
+  else
+    segments([&](float x, int i) { return keep.mass(x, i); });
   __syncthreads();
   uint64_t total = 0;
-  for (int s = 0; s < steps; ++s) total += step_mass[s];
-  uint64_t t = floor_part(total, uniform(a, row));
-  int s = 0;
-  while (t >= step_mass[s]) t -= step_mass[s++];
-  // the thread of that step, then the class of its vector
-  const int i = s * STEP + (int)threadIdx.x * V;
-  const uint64_t own = vec_mass(i), upto = wave_scan(own, threadIdx.x & 63);
-  if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = upto;
-  __syncthreads();
-  uint64_t before = upto - own;
-  for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) before += scratch[w];
-  if (t >= before && t < before + own) {
-    t -= before;
-    for (int e = 0; e < V; ++e) {
-      const float x = (float)z[i + e];
-      const uint32_t key = order_key(x);
-      if (key <= KEY_MASKED || places.of(key, i + e) < cut) continue;
-      const uint64_t w = weight(x, m, c);
-      if (w < least) continue;
-      if (t < w) {
-        a.idx[row] = i + e;
-        a.prob[row] = (float)((double)w / (double)total);
-        break;
-      }
-      t -= w;
-    }
+  const int count = (K + STEP - 1) / STEP * WAVES;
+  crossing<NT, Lds::SEGMENTS / NT>(s.u.segment, count, s.scratch, s.out, [&](uint64_t mass) {
+    total = mass;
+    return floor_part(mass, uniform(a, row)) + 1;  // the first sum above it
+  });
+  const int pick = (int)s.out[0];
+  if (wave != pick % WAVES) return;
+  const uint64_t t = s.out[2] - 1 - s.out[1];
+  Held<T> h;
+  const int i = pick * 64 * V + lane * V;
+  h.load(z, i, K);
+  uint64_t own[V], sum = 0;
+#pragma unroll
+  for (int e = 0; e < V; ++e) sum += own[e] = keep.mass(h[e], i + e);
+  uint64_t before = wave_scan(sum, lane) - sum;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if (t >= before && t < before + own[e]) write_one(a, row, i + e, (float)((double)own[e] / (double)total));
+    before += own[e];
   }
 }
 
@@ -630,20 +548,13 @@ void launch_wave(const SampleCall& a, hipStream_t stream) {
     hipLaunchKernelGGL((sample_wave_kernel<T, NV, false>), grid, dim3(256), 0, stream, a);
 }
 
-template <class T, bool SKIP, int NT, int NV>
-void launch_row(const SampleCall& a, hipStream_t stream) {
-  hipLaunchKernelGGL((sample_row_kernel<T, NT, NV, SKIP>), dim3((unsigned)a.B), dim3(NT), 0, stream, a);
-}
-
 template <class T, bool SKIP>
-void launch_long(const SampleCall& a, hipStream_t stream) {
-  const int vecs = (a.K + Vec<T>::N - 1) / Vec<T>::N;
-  if (vecs <= 256 * 4) return launch_row<T, SKIP, 256, 4>(a, stream);
-  if (vecs <= 512 * 4) return launch_row<T, SKIP, 512, 4>(a, stream);
-  if (vecs <= 1024 * 4) return launch_row<T, SKIP, 1024, 4>(a, stream);
-  if (vecs <= 1024 * 8) return launch_row<T, SKIP, 1024, 8>(a, stream);
-  if (vecs <= 1024 * 16) return launch_row<T, SKIP, 1024, 16>(a, stream);
-  hipLaunchKernelGGL((sample_long_kernel<T, 1024, SKIP>), dim3((unsigned)a.B), dim3(1024), 0, stream, a);
+void launch_row(const SampleCall& a, hipStream_t stream) {
+  const dim3 grid((unsigned)a.B);
+  if (a.K <= SMALL_BLOCK_CLASSES)
+    hipLaunchKernelGGL((sample_row_kernel<T, 256, SKIP>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((sample_row_kernel<T, 1024, SKIP>), grid, dim3(1024), 0, stream, a);
 }
 
 template <class T>
@@ -660,7 +571,7 @@ void run_sample(const SampleCall& a, hipStream_t stream) {
       launch_wave<T, 8>(a, stream);
   } else if (a.top_k != nullptr) {  // each row its own k: the short ones first, the others after
     hipLaunchKernelGGL((sample_list_kernel<T>), dim3((unsigned)a.B), dim3(TOP_THREADS), 0, stream, a);
-    launch_long<T, true>(a, stream);
+    launch_row<T, true>(a, stream);
   } else if (a.top_k_all >= 1 && a.top_k_all <= BLOCK_TOP) {
     const Plan p = make_plan<T>(a);
     if (p.parts == 1) {
@@ -672,7 +583,7 @@ void run_sample(const SampleCall& a, hipStream_t stream) {
       hipLaunchKernelGGL(sample_merge_kernel, dim3((unsigned)a.B), dim3(TOP_THREADS), 0, stream, a, p.parts, lists);
     }
   } else {
-    launch_long<T, false>(a, stream);
+    launch_row<T, false>(a, stream);
   }
   MLAPI_HIP_CHECK(hipGetLastError());
 }
