@@ -90,13 +90,15 @@ __device__ __forceinline__ void draw_from_list(const SampleCall& a, int64_t row,
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int r = i * 64 + lane;
-    own[i] = r < n ? weight(key_logit((uint32_t)(sorted[r] >> places.ib)), keep.m, keep.c) : 0;
+    own[i] = 0;
+    if (i * 64 < n && r < n) own[i] = weight(key_logit((uint32_t)(sorted[r] >> places.ib)), keep.m, keep.c);
     mass += own[i];
   }
   const uint64_t target = set.top_p < 1.f ? ceil_part(wave_sum_int(mass), fmaxf(set.top_p, 0.f)) : ~(uint64_t)0;
   uint64_t before = 0, total = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
+    if (i * 64 >= n) continue;
     const int r = i * 64 + lane;
     const uint64_t upto = before + wave_scan(own[i], lane);
     before = lane_value(upto, 63);
@@ -111,7 +113,7 @@ __device__ __forceinline__ void draw_from_list(const SampleCall& a, int64_t row,
   const uint64_t t = floor_part(total, uniform(a, row));
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    if (i * 64 >= n) break;
+    if (i * 64 >= n) continue;
     const int r = i * 64 + lane, mine = r < n ? c[r] : -1;
     uint64_t lower = 0;  // the kept mass of lower classes
     for (int j = 0; j < n; ++j) lower += c[j] < mine ? w[j] : 0;
@@ -129,6 +131,7 @@ __device__ __forceinline__ void write_one(const SampleCall& a, int64_t row, int 
 
 // ---- one wave, row in registers -------------------------------------------------------------------
 constexpr int WAVE_BINS = 256;
+constexpr int WAVE_LIST = 256;
 struct WaveLds {
   union {
     struct {
@@ -136,6 +139,9 @@ struct WaveLds {
       uint64_t w[WAVE_TOP];
       int c[WAVE_TOP];
     } l;
+    struct {
+      uint64_t mass[WAVE_BINS], place[WAVE_LIST], w[WAVE_LIST];
+    } h;
     SelectLds<WAVE_BINS> select;
   } u;
 };
@@ -184,35 +190,122 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleCall a) {
       draw_from_list<WAVE_TOP>(a, row, set, places, s.u.l.top.sorted, n, lane, s.u.l.w, s.u.l.c);
       return;
     }
-    auto each = [&](auto f) {
-      pass([&](float x, int i) {
+    // every weight once; a class that a filter drops loses its weight
+    uint64_t w[NV * V];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[v * V + e] = keep.any_mass(raw[v][e]);
+    auto each = [&](auto f) {  // f(class, logit, weight)
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int e = 0; e < V; ++e) f((v * 64 + lane) * V + e, raw[v][e], w[v * V + e]);
+    };
+    auto by_place = [&](auto f) {
+      each([&](int i, float x, uint64_t wi) {
         const uint32_t key = order_key(x);
-        if (key > KEY_MASKED) f(places.of(key, i), weight(x, m, keep.c));
+        if (key > KEY_MASKED) f(places.of(key, i), wi);
       });
     };
-    uint64_t lo = places.last(KEY_MASKED + 1);
-    const uint64_t hi = places.first(order_key(m)) - 1;
-    uint64_t mass = 0;
-    bool cut = false;
+    auto cut = [&](uint64_t place) {
+      keep.upto(place, places);
+      each([&](int i, float x, uint64_t& wi) { wi = x > keep.z || (x == keep.z && i <= keep.cls) ? wi : 0; });
+    };
+    const uint64_t lo = places.last(KEY_MASKED + 1), hi = places.first(order_key(m)) - 1;
     if (set.top_k > 0 && set.top_k < K) {
       int valid = 0;
-      pass([&](float x, int) { valid += __popcll(__ballot(x > -__builtin_inff())); });
-      if (set.top_k < valid) {
-        const Prefix p = select_prefix<64, WAVE_BINS>(false, set.top_k, lo, hi, &s.u.select, each);
-        lo = p.cut, mass = p.mass, cut = true;
-      }
+      each([&](int, float x, uint64_t) { valid += __popcll(__ballot(x > -__builtin_inff())); });
+      if (set.top_k < valid)
+        cut(select_prefix<64, WAVE_BINS>(false, set.top_k, lo, hi, &s.u.select, by_place).cut);
     }
     if (set.top_p < 1.f) {
-      if (!cut) {
-        each([&](uint64_t, uint64_t w) { mass += w; });
-        mass = wave_sum_int(mass);
+      uint64_t mass = 0;
+      each([&](int, float, uint64_t wi) { mass += wi; });
+      const uint64_t part = ceil_part(wave_sum_int(mass), fmaxf(set.top_p, 0.f)), target = part == 0 ? 1 : part;
+      // masses by bins of equal width in z, as for a long row (below)
+      constexpr int PER = WAVE_BINS / 64;
+#pragma unroll
+      for (int b = 0; b < PER; ++b) s.u.h.mass[b * 64 + lane] = 0;
+      const float scale = (float)(WAVE_BINS / 30.0) / set.T;
+      auto depth = [&](float x) { return fminf(fmaxf((m - x) * scale, 0.f), (float)(WAVE_BINS - 1)); };
+      auto sync = [] {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      };
+      sync();
+      each([&](int, float x, uint64_t wi) {
+        if (wi != 0) atomicAdd((unsigned long long*)&s.u.h.mass[(int)depth(x)], (unsigned long long)wi);
+      });
+      sync();
+      uint64_t bin[PER], own = 0;
+#pragma unroll
+      for (int b = 0; b < PER; ++b) own += bin[b] = s.u.h.mass[lane * PER + b];
+      const uint64_t upto = wave_scan(own, lane);
+      uint64_t before = upto - own;
+      int at = 0;
+      const uint64_t hit = __ballot(before < target && upto >= target);
+#pragma unroll
+      for (int b = 0; b < PER - 1; ++b)
+        if (before + bin[b] < target && at == b) before += bin[b], ++at;
+      const int where = __builtin_ctzll(hit);
+      const uint64_t above = lane_value(before, where);
+      const float near = (float)lane_value(lane * PER + at, where);
+      int n = 0;
+      each([&](int i, float x, uint64_t wi) {
+        const float d = depth(x);
+        const bool in = wi != 0 && d >= near && d < near + 1.f;
+        const uint64_t mk = __ballot(in);
+        if (mk != 0) {
+          const int j = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mk >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mk, 0));
+          if (in && j < WAVE_LIST) s.u.h.place[j] = places.of(order_key(x), i), s.u.h.w[j] = wi;
+          n += __popcll(mk);
+        }
+      });
+      sync();
+      if (n <= WAVE_LIST) {
+        uint64_t last = 0;
+        for (int j0 = 0; j0 < n; j0 += 64) {
+          const int j = j0 + lane;
+          const uint64_t mine = j < n ? s.u.h.place[j] : 0, wj = j < n ? s.u.h.w[j] : 0;
+          uint64_t sum = above;
+          for (int i = 0; i < n; ++i) sum += s.u.h.place[i] > mine ? s.u.h.w[i] : 0;
+          const uint64_t hits = __ballot(j < n && sum < target && sum + wj >= target);
+          if (hits != 0) last = lane_value(mine, __builtin_ctzll(hits));
+        }
+        cut(last);
+      } else {
+        cut(select_prefix<64, WAVE_BINS>(true, target, lo, hi, &s.u.select, by_place).cut);
       }
-      const uint64_t target = ceil_part(mass, fmaxf(set.top_p, 0.f));
-      lo = select_prefix<64, WAVE_BINS>(true, target == 0 ? 1 : target, lo, hi, &s.u.select, each).cut;
-      cut = true;
     }
-    if (cut) keep.upto(lo, places);
+    each([&](int, float, uint64_t& wi) { wi = wi >= keep.least ? wi : 0; });
+    uint64_t by_vec[NV], total = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      by_vec[v] = 0;
+#pragma unroll
+      for (int e = 0; e < V; ++e) by_vec[v] += w[v * V + e];
+      total += by_vec[v];
+    }
+    total = wave_sum_int(total);
+    const uint64_t t = floor_part(total, uniform(a, row));
+    uint64_t base = 0;  // the kept mass of the vectors before v
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const uint64_t upto = base + wave_scan(by_vec[v], lane);
+      uint64_t before = upto - by_vec[v];
+      base = lane_value(upto, 63);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const uint64_t wi = w[v * V + e];
+        if (t >= before && t < before + wi)
+          write_one(a, row, (v * 64 + lane) * V + e, (float)((double)wi / (double)total));
+        before += wi;
+      }
+    }
+    return;
   }
+  // masses of the lanes' vectors; the weights of the drawn one are computed again
   const bool all = keep.all();
   uint64_t by_vec[NV], total = 0;
 #pragma unroll
