@@ -60,6 +60,40 @@ __device__ __forceinline__ int wave_gather(const Held<T> (&raw)[NV], int lane, P
   return n;
 }
 
+// Where the first k classes of a row in registers end, exactly: they are those with z > over, or z == over
+// and a class of at most `last` (and not masked). The k-th largest key bit by bit, then, among the classes that
+// share it, the last that fits.
+template <class T, int NV>
+__device__ __forceinline__ void wave_cut(const Held<T> (&raw)[NV], int lane, int K, int k, float& over, int& last) {
+  constexpr int V = Vec<T>::N;
+  const Places places(K);
+  auto count = [&](auto pred) {
+    int c = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < V; ++e) c += __popcll(__ballot(pred(raw[v][e], (v * 64 + lane) * V + e)));
+    return c;
+  };
+  const float inf = __builtin_inff();
+  over = -inf, last = K;
+  if (count([&](float z, int) { return z > -inf; }) <= k) return;
+  uint32_t t = 0;
+#pragma unroll 1
+  for (int b = 31; b >= 0; --b) {
+    const float cand = key_logit(t | 1u << b);  // NaN keys: no logit reaches them
+    if (count([&](float z, int) { return z >= cand; }) >= k) t |= 1u << b;
+  }
+  over = key_logit(t);
+  const int ties = k - count([&](float z, int) { return z > over; });
+  last = 0;  // the smallest class by which `ties` classes tie
+#pragma unroll 1
+  for (int b = places.ib - 1; b >= 0; --b) {
+    const int below = last + (1 << b) - 1;
+    if (count([&](float z, int i) { return z == over && i <= below; }) < ties) last += 1 << b;
+  }
+}
+
 // Sorts the first k (at most WAVE_TOP) classes of the row into s->sorted; returns their number.
 template <class T, int NV>
 __device__ __forceinline__ int wave_top(const Held<T> (&raw)[NV], int lane, int K, int k, WaveTopLds* s) {
@@ -85,32 +119,9 @@ __device__ __forceinline__ int wave_top(const Held<T> (&raw)[NV], int lane, int 
   int n = WAVE_CAND + 1;
   if (bound > KEY_MASKED) n = wave_gather<T, NV>(raw, lane, places, key_logit(bound), K, s->cand);
   if (n > WAVE_CAND) {
-    // exactly: the k-th largest key, then (all of its ties need not fit) the class that ends the list
-    auto count = [&](auto pred) {
-      int c = 0;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int e = 0; e < V; ++e) c += __popcll(__ballot(pred(raw[v][e], (v * 64 + lane) * V + e)));
-      return c;
-    };
-    const float inf = __builtin_inff();
-    float over = -inf;
-    int last = K;
-    if (count([&](float z, int) { return z > -inf; }) > k) {
-      uint32_t t = 0;
-      for (int b = 31; b >= 0; --b) {
-        const float cand = key_logit(t | 1u << b);  // NaN keys: no logit reaches them
-        if (count([&](float z, int) { return z >= cand; }) >= k) t |= 1u << b;
-      }
-      over = key_logit(t);
-      const int ties = k - count([&](float z, int) { return z > over; });
-      last = 0;  // the smallest class by which `ties` classes tie
-      for (int b = places.ib - 1; b >= 0; --b) {
-        const int below = last + (1 << b) - 1;
-        if (count([&](float z, int i) { return z == over && i <= below; }) < ties) last += 1 << b;
-      }
-    }
+    float over;
+    int last;
+    wave_cut<T, NV>(raw, lane, K, k, over, last);
     n = wave_gather<T, NV>(raw, lane, places, over, last, s->cand);
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -208,16 +208,13 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleCall a) {
         if (key > KEY_MASKED) f(places.of(key, i), wi);
       });
     };
-    auto cut = [&](uint64_t place) {
-      keep.upto(place, places);
+    auto drop = [&] {  // what lies past the last class kept
       each([&](int i, float x, uint64_t& wi) { wi = x > keep.z || (x == keep.z && i <= keep.cls) ? wi : 0; });
     };
     const uint64_t lo = places.last(KEY_MASKED + 1), hi = places.first(order_key(m)) - 1;
     if (set.top_k > 0 && set.top_k < K) {
-      int valid = 0;
-      each([&](int, float x, uint64_t) { valid += __popcll(__ballot(x > -__builtin_inff())); });
-      if (set.top_k < valid)
-        cut(select_prefix<64, WAVE_BINS>(false, set.top_k, lo, hi, &s.u.select, by_place).cut);
+      wave_cut<T, NV>(raw, lane, K, set.top_k, keep.z, keep.cls);
+      drop();
     }
     if (set.top_p < 1.f) {
       uint64_t mass = 0;
@@ -273,10 +270,11 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleCall a) {
           const uint64_t hits = __ballot(j < n && sum < target && sum + wj >= target);
           if (hits != 0) last = lane_value(mine, __builtin_ctzll(hits));
         }
-        cut(last);
+        keep.upto(last, places);
       } else {
-        cut(select_prefix<64, WAVE_BINS>(true, target, lo, hi, &s.u.select, by_place).cut);
+        keep.upto(select_prefix<64, WAVE_BINS>(true, target, lo, hi, &s.u.select, by_place).cut, places);
       }
+      drop();
     }
     each([&](int, float, uint64_t& wi) { wi = wi >= keep.least ? wi : 0; });
     uint64_t by_vec[NV], total = 0;

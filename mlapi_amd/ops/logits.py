@@ -23,10 +23,31 @@ import torch
 from mlapi_amd._native import C
 
 _DT = {torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
+MAX_CLASSES, MAX_TOP = 1 << 20, 1024  # the launchers' LOGIT_MAX_CLASSES, LOGIT_MAX_TOP
+
+# The current stream of a device as a number: 0.06 us where a torch.cuda.Stream takes 1.8, of the 7 us that a
+# call on a small batch spends on the host.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+class _On:
+    """Launch on a tensor's device, whichever is current: ``with _On(Z) as stream``."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+
+    def __enter__(self) -> int:
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return _raw_stream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
 
 
 def _logits(name: str, Z: torch.Tensor) -> Tuple[int, int, int]:
@@ -38,8 +59,8 @@ def _logits(name: str, Z: torch.Tensor) -> Tuple[int, int, int]:
     if Z.dim() != 2 or Z.shape[1] < 1:
         raise ValueError(f"{name}: logits must be [B, K] with K >= 1")
     B, K = Z.shape
-    if K > C().LOGIT_MAX_CLASSES:
-        raise ValueError(f"{name}: at most {C().LOGIT_MAX_CLASSES} classes (got {K})")
+    if K > MAX_CLASSES:
+        raise ValueError(f"{name}: at most {MAX_CLASSES} classes (got {K})")
     if K > 1 and Z.stride(1) != 1:
         raise ValueError(f"{name}: the classes of a row must be contiguous")
     ld = Z.stride(0) if B > 1 else K
@@ -63,8 +84,12 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + n * t.element_size()
 
 
-def _workspace(nbytes: int, device) -> torch.Tensor:
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+def _workspace(nbytes: int, device) -> Tuple[Optional[torch.Tensor], int]:
+    """(the tensor that keeps it alive, its address)"""
+    if nbytes == 0:
+        return None, 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr()
 
 
 # -------------------------------------------------------------------------------------------- top
@@ -75,36 +100,41 @@ def top_logits(Z: torch.Tensor, k: int, out: Optional[Tuple[torch.Tensor, torch.
     writes into preallocated contiguous tensors."""
     B, K, ld = _logits("top_logits", Z)
     k = int(k)
-    if not 1 <= k <= C().LOGIT_MAX_TOP:
-        raise ValueError(f"top_logits: k must be in [1, {C().LOGIT_MAX_TOP}] (got {k})")
+    if not 1 <= k <= MAX_TOP:
+        raise ValueError(f"top_logits: k must be in [1, {MAX_TOP}] (got {k})")
     if out is None:
-        out = (torch.empty(B, k, dtype=Z.dtype, device=Z.device), torch.empty(B, k, dtype=torch.int32, device=Z.device))
-    values, idx = out
-    for t, dt in ((values, Z.dtype), (idx, torch.int32)):
-        if t.dtype != dt or t.shape != (B, k) or not t.is_contiguous() or t.device != Z.device:
-            raise ValueError("top_logits: out must be contiguous (Z's type [B, k], int32 [B, k]) on Z's device")
+        values = torch.empty((B, k), dtype=Z.dtype, device=Z.device)
+        idx = torch.empty((B, k), dtype=torch.int32, device=Z.device)
+    else:
+        values, idx = out
+        for t, dt in ((values, Z.dtype), (idx, torch.int32)):
+            if t.dtype != dt or t.shape != (B, k) or not t.is_contiguous() or t.device != Z.device:
+                raise ValueError("top_logits: out must be contiguous (Z's type [B, k], int32 [B, k]) on Z's device")
     dt = _DT[Z.dtype]
-    with torch.cuda.device(Z.device):
-        ws = _workspace(C().top_logits_workspace(dt, B, K, k), Z.device)
-        C().top_logits(dt, Z.data_ptr(), ld, B, K, k, values.data_ptr(), idx.data_ptr(), ws.data_ptr(), ws.numel(),
-                       _stream(Z.device))
+    c = C()
+    with _On(Z) as stream:
+        n = c.top_logits_workspace(dt, B, K, k)
+        ws, at = _workspace(n, Z.device)
+        c.top_logits(dt, Z.data_ptr(), ld, B, K, k, values.data_ptr(), idx.data_ptr(), at, n, stream)
     return values, idx
 
 
 # ------------------------------------------------------------------------------------ distillation
-def _distill(name: str, Z, idx, t, temperature, alpha, y, *, g=None, stats_in=None, loss=None, stats_out=None,
-             pred=None, dz=None) -> None:
+def _distill(name: str, Z, idx, t, temperature, alpha, y, *, g=None, stats_in=None, loss=False, stats=False, pred=None,
+             dz=None, out=None):
+    """One call: (loss, statistics) where asked for; the gradient goes to ``out``, or with ``dz`` to a new tensor."""
     B, K, ld = _logits(name, Z)
+    dev = Z.device
     for what, v in (("idx", idx), ("t", t)):
-        if not isinstance(v, torch.Tensor) or v.device != Z.device:
-            raise ValueError(f"{name}: {what} must be a tensor on {Z.device}")
+        if not isinstance(v, torch.Tensor) or v.device != dev:
+            raise ValueError(f"{name}: {what} must be a tensor on {dev}")
         if v.dim() != 2 or v.shape[0] != B or v.shape[1] < 1 or (v.shape[1] > 1 and v.stride(1) != 1):
             raise ValueError(f"{name}: {what} must be [B, k], k >= 1, with contiguous rows")
     if idx.dtype != torch.int32 or t.dtype not in _DT:
         raise TypeError(f"{name}: idx must be int32 and t f32, bf16 or f16")
     k = idx.shape[1]
-    if t.shape[1] != k or k > C().LOGIT_MAX_TOP:
-        raise ValueError(f"{name}: idx and t must both be [B, k], k <= {C().LOGIT_MAX_TOP}")
+    if t.shape[1] != k or k > MAX_TOP:
+        raise ValueError(f"{name}: idx and t must both be [B, k], k <= {MAX_TOP}")
     temperature, alpha = float(temperature), float(alpha)
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError(f"{name}: temperature must be in [1e-6, 1e6] (got {temperature})")
@@ -114,25 +144,38 @@ def _distill(name: str, Z, idx, t, temperature, alpha, y, *, g=None, stats_in=No
         raise ValueError(f"{name}: alpha below 1 mixes in hard labels and needs y")
     yp = 0 if y is None else _vector(name, "y", y, Z, torch.int32)
     gp = 0 if g is None else _vector(name, "g", g, Z, torch.float32)
-    ldd, ddt = 0, _DT[Z.dtype]
-    if dz is not None:
-        if not isinstance(dz, torch.Tensor) or dz.device != Z.device or dz.shape != Z.shape or dz.dtype not in (
+    pp = 0 if pred is None else _vector(name, "pred", pred, Z, torch.int32)
+    dt = ddt = _DT[Z.dtype]
+    ldd = dp = 0
+    if out is not None:
+        if not isinstance(out, torch.Tensor) or out.device != dev or out.shape != Z.shape or out.dtype not in (
                 Z.dtype, *((torch.bfloat16,) if Z.dtype == torch.float32 else ())):
             raise ValueError(f"{name}: out must be [B, K] on Z's device in Z's type (or bf16 for f32 logits)")
-        ldd = dz.stride(0) if B > 1 else K
-        if (K > 1 and dz.stride(1) != 1) or ldd < K:
+        ldd = out.stride(0) if B > 1 else K
+        if (K > 1 and out.stride(1) != 1) or ldd < K:
             raise ValueError(f"{name}: out must have contiguous, separate rows")
-        ddt = _DT[dz.dtype]
-        (a, b), (c, d) = _span(Z), _span(dz)
-        if a < d and c < b and not (a == c and ld == ldd and Z.dtype == dz.dtype):
-            raise ValueError(f"{name}: out overlaps the logits without being the logits")
-    ptr = lambda v: 0 if v is None else v.data_ptr()  # noqa: E731
-    dt = _DT[Z.dtype]
-    with torch.cuda.device(Z.device):
-        ws = _workspace(0 if stats_in is not None else C().distill_workspace(dt, B, K), Z.device)
-        C().distill(dt, _DT[t.dtype], ddt, Z.data_ptr(), ld, B, K, idx.data_ptr(), idx.stride(0) if B > 1 else k,
-                    t.data_ptr(), t.stride(0) if B > 1 else k, k, temperature, alpha, yp, gp, ptr(stats_in), ptr(loss),
-                    ptr(stats_out), ptr(pred), ptr(dz), ldd, ws.data_ptr(), ws.numel(), _stream(Z.device))
+        ddt, dp = _DT[out.dtype], out.data_ptr()
+        same = dp == Z.data_ptr() and ld == ldd and Z.dtype == out.dtype
+        for what, v in (("the logits without being the logits", Z), ("idx", idx), ("t", t), ("y", y), ("g", g),
+                        ("stats", stats_in), ("pred", pred)):
+            if v is not None and not (v is Z and same):
+                (a, b), (p, q) = _span(v), _span(out)
+                if a < q and p < b:
+                    raise ValueError(f"{name}: out overlaps {what}")
+    elif dz:
+        out = torch.empty((B, K), dtype=Z.dtype, device=dev)
+        ldd, dp = K, out.data_ptr()
+    loss = torch.empty(B, dtype=torch.float32, device=dev) if loss else None
+    stats = torch.empty((B, 4), dtype=torch.float32, device=dev) if stats else None
+    c = C()
+    with _On(Z) as stream:
+        n = 0 if stats_in is not None else c.distill_workspace(dt, B, K)
+        ws, at = _workspace(n, dev)
+        c.distill(dt, _DT[t.dtype], ddt, Z.data_ptr(), ld, B, K, idx.data_ptr(), idx.stride(0) if B > 1 else k,
+                  t.data_ptr(), t.stride(0) if B > 1 else k, k, temperature, alpha, yp, gp,
+                  0 if stats_in is None else stats_in.data_ptr(), 0 if loss is None else loss.data_ptr(),
+                  0 if stats is None else stats.data_ptr(), pp, dp, ldd, at, n, stream)
+    return loss, stats, out
 
 
 def distill_loss(Z: torch.Tensor, idx: torch.Tensor, t: torch.Tensor, *, temperature: float = 1.0, alpha: float = 1.0,
@@ -148,10 +191,7 @@ def distill_loss(Z: torch.Tensor, idx: torch.Tensor, t: torch.Tensor, *, tempera
     A row without entries has no first part, a row with y < 0 no second, a row whose logits are all -inf
     neither. A listed class that the student masks makes the loss +inf. A class >= K in idx or y makes its
     row's loss and gradient NaN."""
-    B = _logits("distill_loss", Z)[0]
-    loss = torch.empty(B, dtype=torch.float32, device=Z.device)
-    stats = torch.empty(B, 4, dtype=torch.float32, device=Z.device)
-    _distill("distill_loss", Z, idx, t, temperature, alpha, y, loss=loss, stats_out=stats)
+    loss, stats, _ = _distill("distill_loss", Z, idx, t, temperature, alpha, y, loss=True, stats=True)
     return loss, stats
 
 
@@ -161,13 +201,10 @@ def distill_grad(Z: torch.Tensor, idx: torch.Tensor, t: torch.Tensor, stats: tor
     """d(sum_r g_r loss_r)/dZ, [B, K] in Z's type, from the statistics :func:`distill_loss` gave for the same
     arguments. ``g`` f32 [B] weights the rows (None: 1). ``out``: where to write it - any row stride, bf16 for f32
     logits, or Z itself. The teacher's logits get no gradient."""
-    B = _logits("distill_grad", Z)[0]
-    if not isinstance(stats, torch.Tensor) or stats.device != Z.device or stats.dtype != torch.float32 or \
-            stats.shape != (B, 4) or not stats.is_contiguous():
+    if not isinstance(Z, torch.Tensor) or not isinstance(stats, torch.Tensor) or stats.device != Z.device or \
+            stats.dtype != torch.float32 or stats.shape != (Z.shape[0], 4) or not stats.is_contiguous():
         raise ValueError("distill_grad: stats must be the [B, 4] statistics of distill_loss")
-    dz = torch.empty(Z.shape, dtype=Z.dtype, device=Z.device) if out is None else out
-    _distill("distill_grad", Z, idx, t, temperature, alpha, y, g=g, stats_in=stats, dz=dz)
-    return dz
+    return _distill("distill_grad", Z, idx, t, temperature, alpha, y, g=g, stats_in=stats, dz=True, out=out)[2]
 
 
 def distill_loss_grad(Z: torch.Tensor, idx: torch.Tensor, t: torch.Tensor, *, g: Optional[torch.Tensor] = None,
@@ -176,17 +213,23 @@ def distill_loss_grad(Z: torch.Tensor, idx: torch.Tensor, t: torch.Tensor, *, g:
                       ) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`distill_loss` and :func:`distill_grad` in one pass over the logits: (loss f32 [B], dZ). ``g`` weights the
     gradient alone. ``pred`` int32 [B], if given, receives every row's first maximum."""
-    B = _logits("distill_loss_grad", Z)[0]
-    loss = torch.empty(B, dtype=torch.float32, device=Z.device)
-    dz = torch.empty(Z.shape, dtype=Z.dtype, device=Z.device) if out is None else out
-    if pred is not None:
-        _vector("distill_loss_grad", "pred", pred, Z, torch.int32)
-    _distill("distill_loss_grad", Z, idx, t, temperature, alpha, y, g=g, loss=loss, pred=pred, dz=dz)
+    loss, _, dz = _distill("distill_loss_grad", Z, idx, t, temperature, alpha, y, g=g, loss=True, pred=pred, dz=True,
+                           out=out)
     return loss, dz
 
 
 # ---------------------------------------------------------------------------------------- sampling
 Setting = Union[float, int, torch.Tensor]
+
+
+def _setting(name: str, v: Setting, Z: torch.Tensor, dtype: torch.dtype, number, most: float):
+    """(address of a per-row setting or 0, the number for all rows)"""
+    if isinstance(v, torch.Tensor):
+        return _vector("sample_logits", name, v, Z, dtype), 0
+    n = number(v)
+    if not 0 <= n <= most:
+        raise ValueError(f"sample_logits: {name} must be in [0, {most}] (got {v})")
+    return 0, n
 
 
 def sample_logits(Z: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0, top_k: Setting = 0,
@@ -206,29 +249,23 @@ def sample_logits(Z: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.
     always draw the same class."""
     B, K, ld = _logits("sample_logits", Z)
     up = _vector("sample_logits", "u", u, Z, torch.float32)
-    ptrs, nums = {}, {}
-    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if isinstance(v, torch.Tensor):
-            ptrs[name], nums[name] = _vector("sample_logits", name, v, Z, dtype), 0
-        else:
-            ptrs[name], nums[name] = 0, int(v) if name == "top_k" else float(v)
-    if not nums["temperature"] >= 0.0:
-        raise ValueError(f"sample_logits: temperature must be >= 0 (got {temperature})")
-    if nums["top_k"] < 0:
-        raise ValueError(f"sample_logits: top_k must be >= 0 (got {top_k})")
-    if not 0.0 <= nums["top_p"] <= 1.0 or not 0.0 <= nums["min_p"] <= 1.0:
-        raise ValueError(f"sample_logits: top_p and min_p must be in [0, 1] (got {top_p}, {min_p})")
-    nums["top_k"] = min(nums["top_k"], K)
+    Tp, T = _setting("temperature", temperature, Z, torch.float32, float, float("inf"))
+    kp, k = _setting("top_k", top_k, Z, torch.int32, int, float("inf"))
+    pp, p = _setting("top_p", top_p, Z, torch.float32, float, 1.0)
+    mp, least = _setting("min_p", min_p, Z, torch.float32, float, 1.0)
+    k = min(k, K)
     if out is None:
-        out = (torch.empty(B, dtype=torch.int32, device=Z.device), torch.empty(B, dtype=torch.float32, device=Z.device))
-    idx, prob = out
-    _vector("sample_logits", "out idx", idx, Z, torch.int32)
-    _vector("sample_logits", "out prob", prob, Z, torch.float32)
+        idx = torch.empty(B, dtype=torch.int32, device=Z.device)
+        prob = torch.empty(B, dtype=torch.float32, device=Z.device)
+    else:
+        idx, prob = out
+        _vector("sample_logits", "out idx", idx, Z, torch.int32)
+        _vector("sample_logits", "out prob", prob, Z, torch.float32)
     dt = _DT[Z.dtype]
-    with torch.cuda.device(Z.device):
-        ws = _workspace(C().sample_workspace(dt, B, K, ptrs["top_k"] != 0, nums["top_k"]), Z.device)
-        C().sample_logits(dt, Z.data_ptr(), ld, B, K, up, ptrs["temperature"], nums["temperature"], ptrs["top_k"],
-                          nums["top_k"], ptrs["top_p"], nums["top_p"], ptrs["min_p"], nums["min_p"], idx.data_ptr(),
-                          prob.data_ptr(), ws.data_ptr(), ws.numel(), _stream(Z.device))
+    c = C()
+    with _On(Z) as stream:
+        n = c.sample_workspace(dt, B, K, kp != 0, k)
+        ws, at = _workspace(n, Z.device)
+        c.sample_logits(dt, Z.data_ptr(), ld, B, K, up, Tp, T, kp, k, pp, p, mp, least, idx.data_ptr(),
+                        prob.data_ptr(), at, n, stream)
     return idx, prob
