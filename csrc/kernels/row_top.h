@@ -28,11 +28,39 @@ __device__ __forceinline__ U kth_largest(const U (&v)[M], int k, int bits) {
   return t;
 }
 
+// Ranks n distinct places in LDS (by how many are larger) over THREADS threads, each holding PER of them:
+// sorted[r] gets the place of rank r < k. Every place is read once by all, four at a time: `cand` is padded
+// with zeros to a multiple of four.
+template <int THREADS, int PER>
+__device__ __forceinline__ void rank_some(const uint64_t* cand, int n, int k, int tid, uint64_t* sorted) {
+  uint64_t mine[PER];
+  int rank[PER];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) mine[p] = tid + p * THREADS < n ? cand[tid + p * THREADS] : ~(uint64_t)0, rank[p] = 0;
+#pragma unroll 1
+  for (int i = 0; i < n; i += 4) {
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(cand + i), y = *reinterpret_cast<const ulonglong2*>(cand + i + 2);
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      rank[p] += (x.x > mine[p] ? 1 : 0) + (x.y > mine[p] ? 1 : 0) + (y.x > mine[p] ? 1 : 0) + (y.y > mine[p] ? 1 : 0);
+  }
+#pragma unroll
+  for (int p = 0; p < PER; ++p)
+    if (tid + p * THREADS < n && rank[p] < k) sorted[rank[p]] = mine[p];
+}
+// n is the same for all threads
+template <int THREADS, int MOST>
+__device__ __forceinline__ void rank_places(const uint64_t* cand, int n, int k, int tid, uint64_t* sorted) {
+  if (n <= THREADS) return rank_some<THREADS, 1>(cand, n, k, tid, sorted);
+  if (n <= 2 * THREADS) return rank_some<THREADS, 2>(cand, n, k, tid, sorted);
+  rank_some<THREADS, MOST>(cand, n, k, tid, sorted);
+}
+
 // ---- one wave, row in registers -----------------------------------------------------------------
 constexpr int WAVE_TOP = 256;   // longest list
 constexpr int WAVE_CAND = 512;  // gathered classes
-struct WaveTopLds {
-  uint64_t cand[WAVE_CAND];
+struct alignas(16) WaveTopLds {
+  uint64_t cand[WAVE_CAND + 4];
   uint64_t sorted[WAVE_TOP];
 };
 
@@ -124,14 +152,11 @@ __device__ __forceinline__ int wave_top(const Held<T> (&raw)[NV], int lane, int 
     wave_cut<T, NV>(raw, lane, K, k, over, last);
     n = wave_gather<T, NV>(raw, lane, places, over, last, s->cand);
   }
+  n = __builtin_amdgcn_readfirstlane(n);
+  if (lane < 4) s->cand[n + lane] = 0;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  for (int j = lane; j < n; j += 64) {
-    const uint64_t mine = s->cand[j];
-    int r = 0;
-    for (int i = 0; i < n; ++i) r += s->cand[i] > mine ? 1 : 0;
-    if (r < k) s->sorted[r] = mine;
-  }
+  rank_places<64, WAVE_CAND / 64>(s->cand, n, k, lane, s->sorted);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
   return min(n, k);
@@ -143,7 +168,8 @@ constexpr int BLOCK_TOP = 128;    // longest list
 constexpr int BLOCK_CAND = 1024;  // gathered classes
 constexpr int GROUP_LANES = 16;   // a group is 16 lanes' vectors of `rounds` steps: 256 bytes each
 constexpr int MAX_GROUPS = 2048;
-struct BlockTopLds {
+struct alignas(16) BlockTopLds {
+  uint64_t cand[BLOCK_CAND + 4];
   union {
     struct {
       float most[MAX_GROUPS];
@@ -151,7 +177,6 @@ struct BlockTopLds {
     } g;
     SelectLds<SELECT_BINS> select;
   } u;
-  uint64_t cand[BLOCK_CAND];
   uint64_t sorted[BLOCK_TOP];
   uint64_t best[TOP_THREADS];
   int groups, n;
@@ -159,13 +184,10 @@ struct BlockTopLds {
 
 // ranks the s->n gathered places
 __device__ __forceinline__ int block_rank(int k, BlockTopLds* s) {
-  const int n = s->n;
-  for (int j = threadIdx.x; j < n; j += TOP_THREADS) {
-    const uint64_t mine = s->cand[j];
-    int r = 0;
-    for (int i = 0; i < n; ++i) r += s->cand[i] > mine ? 1 : 0;
-    if (r < k) s->sorted[r] = mine;
-  }
+  const int n = __builtin_amdgcn_readfirstlane(s->n);
+  if (threadIdx.x < 4) s->cand[n + threadIdx.x] = 0;
+  __syncthreads();
+  rank_places<TOP_THREADS, BLOCK_CAND / TOP_THREADS>(s->cand, n, k, threadIdx.x, s->sorted);
   __syncthreads();
   return min(n, k);
 }

@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <stdexcept>
+#include <type_traits>
 
 #include "kernels/row_top.h"
 #include "mlapi/common.h"
@@ -84,6 +85,7 @@ __device__ __forceinline__ Keep keep_all(float m, const Settings& set) {
 template <int MAX>
 __device__ __forceinline__ void draw_from_list(const SampleCall& a, int64_t row, const Settings& set, Places places,
                                const uint64_t* sorted, int n, int lane, uint64_t* w, int* c) {
+  n = __builtin_amdgcn_readfirstlane(n);
   constexpr int PER = MAX / 64;
   const Keep keep = keep_all(key_logit((uint32_t)(sorted[0] >> places.ib)), set);
   uint64_t own[PER], mass = 0;
@@ -111,17 +113,30 @@ __device__ __forceinline__ void draw_from_list(const SampleCall& a, int64_t row,
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
   const uint64_t t = floor_part(total, uniform(a, row));
+  auto pick = [&](auto rounds) {
+    constexpr int R = decltype(rounds)::value;
+    int mine[R];
+    uint64_t lower[R];  // the kept mass of lower classes
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if (i * 64 >= n) continue;
-    const int r = i * 64 + lane, mine = r < n ? c[r] : -1;
-    uint64_t lower = 0;  // the kept mass of lower classes
-    for (int j = 0; j < n; ++j) lower += c[j] < mine ? w[j] : 0;
-    if (own[i] != 0 && lower <= t && t < lower + own[i]) {
-      a.idx[row] = mine;
-      a.prob[row] = (float)((double)own[i] / (double)total);
+    for (int i = 0; i < R; ++i) mine[i] = i * 64 + lane < n ? c[i * 64 + lane] : -1, lower[i] = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const uint64_t wj = w[j];
+      const int cj = c[j];
+#pragma unroll
+      for (int i = 0; i < R; ++i) lower[i] += cj < mine[i] ? wj : 0;
     }
-  }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (own[i] != 0 && lower[i] <= t && t < lower[i] + own[i]) {
+        a.idx[row] = mine[i];
+        a.prob[row] = (float)((double)own[i] / (double)total);
+      }
+  };
+  if (n <= 64)
+    pick(std::integral_constant<int, 1>{});
+  else
+    pick(std::integral_constant<int, PER>{});
 }
 
 __device__ __forceinline__ void write_one(const SampleCall& a, int64_t row, int cls, float prob) {
@@ -132,12 +147,13 @@ __device__ __forceinline__ void write_one(const SampleCall& a, int64_t row, int 
 // ---- one wave, row in registers -------------------------------------------------------------------
 constexpr int WAVE_BINS = 256;
 constexpr int WAVE_LIST = 256;
+constexpr int WAVE_SHORT = 64;  // longest top-k by a list: 64 rows of 1000, k = 50: 9 us (20 at 128), by a cut 16 at any k
 struct WaveLds {
   union {
     struct {
       WaveTopLds top;
-      uint64_t w[WAVE_TOP];
-      int c[WAVE_TOP];
+      uint64_t w[WAVE_SHORT];
+      int c[WAVE_SHORT];
     } l;
     struct {
       uint64_t mass[WAVE_BINS], place[WAVE_LIST], w[WAVE_LIST];
@@ -185,9 +201,9 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleCall a) {
   if constexpr (!ALL) {
     WaveLds& s = lds[wave];
     const Places places(K);
-    if (set.top_k > 0 && set.top_k <= WAVE_TOP) {
+    if (set.top_k > 0 && set.top_k <= WAVE_SHORT) {
       const int n = wave_top<T, NV>(raw, lane, K, set.top_k, &s.u.l.top);
-      draw_from_list<WAVE_TOP>(a, row, set, places, s.u.l.top.sorted, n, lane, s.u.l.w, s.u.l.c);
+      draw_from_list<WAVE_SHORT>(a, row, set, places, s.u.l.top.sorted, n, lane, s.u.l.w, s.u.l.c);
       return;
     }
     // every weight once; a class that a filter drops loses its weight
@@ -266,6 +282,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(SampleCall a) {
           const int j = j0 + lane;
           const uint64_t mine = j < n ? s.u.h.place[j] : 0, wj = j < n ? s.u.h.w[j] : 0;
           uint64_t sum = above;
+#pragma unroll 4
           for (int i = 0; i < n; ++i) sum += s.u.h.place[i] > mine ? s.u.h.w[i] : 0;
           const uint64_t hits = __ballot(j < n && sum < target && sum + wj >= target);
           if (hits != 0) last = lane_value(mine, __builtin_ctzll(hits));
@@ -556,6 +573,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleCall a) {
       for (int j = tid; j < n; j += NT) {
         const uint64_t mine = s.u.h.place[j], w = s.u.h.w[j];
         uint64_t before = above;
+#pragma unroll 4
         for (int i = 0; i < n; ++i) before += s.u.h.place[i] > mine ? s.u.h.w[i] : 0;
         if (before < target && before + w >= target) s.out[0] = mine;
       }
