@@ -318,6 +318,16 @@ void launch_softmax_grad_wide(const void* X_aug, int64_t ldx, const void* W, con
                               size_t ws_bytes, hipStream_t stream, const Sgd2D* update = nullptr,
                               P2PAllReduce* dp = nullptr, int dp_timeout_ms = 0);
 
+// The step's G^T X launch alone: dW slabs[row_groups][K][F + 8] = G^T X_aug for any G bf16 [B][Kp] (columns
+// past K are not used) and any F; launch_gdw_reduce sums the slabs.
+struct GtxPlan {
+  int Kp, row_groups;
+  int64_t rows_per_group;
+};
+GtxPlan gtx_plan(int64_t B, int K, int F);
+void launch_gtx(const uint16_t* G, const GtxPlan& plan, const void* X_aug, int64_t ldx, int64_t B, int F, int K,
+                float* slabs, hipStream_t stream);
+
 // ---- train kernels (train.hip) -----------------------------------------------------------------
 // Binary logistic regression, one pass over X: accumulates grad (F w-entries, 1 bias) and stats
 // [loss_sum, n_correct] into per-block slabs, then reduce_slabs() folds them into out[F + 3]:
@@ -391,6 +401,17 @@ struct DistillCall {
 };
 size_t distill_workspace(int dt, int64_t B, int K);
 void launch_distill(const DistillCall& call, hipStream_t stream);
+
+// Distillation step of the multiclass trainer (softmax_distill.hip): logits of X_aug (its first F columns)
+// and W, launch_distill's loss and gradient G in bf16, dW_aug = G^T X_aug, the slab sum with the optional
+// update and exchange as in launch_softmax_grad_wide. stats_out = [loss_sum, n_correct] (0 correct
+// without y). F: a width launch_gemm_logits_ld takes. Workspace: softmax_distill_workspace bytes.
+size_t softmax_distill_workspace(int64_t B, int K, int F);
+void launch_softmax_distill(const void* X_aug, int64_t ldx, const void* W, const float* b, const int32_t* idx,
+                            int64_t ldi, const void* t, int64_t ldt, int t_dt, int k, float temperature, float alpha,
+                            const int32_t* y, int64_t B, int F, int K, float* dW_out, float* stats_out, void* workspace,
+                            size_t ws_bytes, hipStream_t stream, const Sgd2D* update = nullptr,
+                            P2PAllReduce* dp = nullptr, int dp_timeout_ms = 0);
 
 // One class drawn per row (definition: sample.hip): u f32 [B]; each setting a device array [B] or,
 // where that is null, one value for all rows. idx int32 [B] (-1: no class), prob f32 [B].

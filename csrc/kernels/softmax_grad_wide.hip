@@ -202,14 +202,10 @@ __global__ __launch_bounds__(256) void gdw_gemm_dma_kernel(const uint16_t* __res
     }
 }
 
-struct WideLayout {
-  size_t g_off, dw_off, stat_off, z_off, wp_off, total;
-  int Kp, row_groups, g_blocks;
-  int64_t rows_per_group;
-};
+}  // namespace
 
-WideLayout wide_layout(int64_t B, int K, int F) {
-  WideLayout L{};
+GtxPlan gtx_plan(int64_t B, int K, int F) {
+  GtxPlan L{};
   const int F_aug = F + 8;
   const int T = 128;  // G's columns padded to the class tile
   L.Kp = (K + T - 1) / T * T;
@@ -234,6 +230,33 @@ WideLayout wide_layout(int64_t B, int K, int F) {
   if (rg < 1) rg = 1;
   L.rows_per_group = ((B + rg - 1) / rg + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
   L.row_groups = (int)((B + L.rows_per_group - 1) / L.rows_per_group);
+  return L;
+}
+
+void launch_gtx(const uint16_t* G, const GtxPlan& L, const void* X_aug, int64_t ldx, int64_t B, int F, int K,
+                float* slabs, hipStream_t stream) {
+  if (L.rows_per_group * ldx * 2 > (int64_t)INT32_MAX)
+    throw std::invalid_argument("softmax_grad_wide: X_aug row stride too large for a row group's 32-bit offsets");
+  const int F_aug = F + 8;
+  const int ncb = L.Kp / 128, nfb = (F_aug + TF128 - 1) / TF128;
+  const int rounds = (L.row_groups + 7) / 8;
+  hipLaunchKernelGGL((gdw_gemm_dma_kernel<3>), dim3((unsigned)(8 * ncb * nfb * rounds)), dim3(256), 0, stream, G, L.Kp,
+                     static_cast<const uint16_t*>(X_aug), ldx, F_aug, B, K, L.rows_per_group, slabs, ncb * nfb,
+                     L.row_groups);
+  MLAPI_HIP_CHECK(hipGetLastError());
+}
+
+namespace {
+
+struct WideLayout : GtxPlan {
+  size_t g_off, dw_off, stat_off, z_off, wp_off, total;
+  int g_blocks;
+};
+
+WideLayout wide_layout(int64_t B, int K, int F) {
+  WideLayout L{};
+  static_cast<GtxPlan&>(L) = gtx_plan(B, K, F);
+  const int F_aug = F + 8;
   L.g_blocks = softmax_rows_g_blocks(B, F, K);  // the row-stats launch's {loss, correct} slabs
   auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
   size_t o = 0;
@@ -298,12 +321,7 @@ void launch_softmax_grad_wide(const void* X_aug, int64_t ldx, const void* W, con
   launch_softmax_rows_g(X_aug, ldx, W, b, y, B, F, K, kind, G, L.Kp, stat_slabs, Zs, wp, stream);
   const int g_blocks = L.g_blocks;
   const int F_aug = F + 8;
-  const int ncb = L.Kp / 128, nfb = (F_aug + TF128 - 1) / TF128;
-  const int rounds = (L.row_groups + 7) / 8;
-  hipLaunchKernelGGL((gdw_gemm_dma_kernel<3>), dim3((unsigned)(8 * ncb * nfb * rounds)), dim3(256), 0, stream, G, L.Kp,
-                     static_cast<const uint16_t*>(X_aug), ldx, F_aug, B, K, L.rows_per_group, slabs, ncb * nfb,
-                     L.row_groups);
-  MLAPI_HIP_CHECK(hipGetLastError());
+  launch_gtx(G, L, X_aug, ldx, B, F, K, slabs, stream);
   launch_gdw_reduce(slabs, L.row_groups, K, F_aug, dW_out, stat_slabs, g_blocks, stats_out, update, dp,
                     dp_timeout_ms, stream);
 }

@@ -44,6 +44,7 @@ SOURCES = [
     "kernels/top_logits.hip",
     "kernels/distill.hip",
     "kernels/sample.hip",
+    "kernels/softmax_distill.hip",
     "runtime/engine.cpp",
     "runtime/direct_dispatch.cpp",
     "http/server.cpp",

@@ -168,6 +168,52 @@ class LogisticRegression:
     def predict(self, X) -> np.ndarray:
         return self._m().classes[self.predict_max(X)[0]]
 
+    def _class_logits(self, X):
+        import torch
+
+        return torch.as_tensor(self._m().class_logits(X), dtype=torch.float32, device=self._torch_device())
+
+    def predict_top(self, X, k: int):
+        """The k most likely classes of every row, likeliest first: (labels [n, k], f32 logits [n, k]; their softmax
+        over all classes is :meth:`predict_proba`). ``k`` is at most the number of classes."""
+        if not 1 <= int(k) <= self._m().n_classes:
+            raise ValueError(f"k must be in [1, {self._m().n_classes}] (got {k})")
+        Z = self._class_logits(X)
+        if Z.is_cuda:
+            from mlapi_amd.ops.logits import top_logits
+
+            v, i = top_logits(Z, int(k))
+        else:
+            from mlapi_amd.ops.reference import top_logits_ref
+
+            v, i = top_logits_ref(Z, int(k))
+        return self._m().classes[i.cpu().numpy()], v.cpu().numpy()
+
+    def sample(self, X, u=None, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
+        """A class drawn for every row from its predicted distribution: (labels [n], their probability among the
+        classes the filters keep). ``u``: one random number in [0, 1) per row (None: drawn with ``random_state``);
+        temperature and filters as in :func:`mlapi_amd.ops.logits.sample_logits`. Temperature 0 is :meth:`predict`."""
+        import torch
+
+        Z = self._class_logits(X)
+        if u is None:
+            u = np.random.default_rng(self.random_state).random(Z.shape[0])
+        u = torch.as_tensor(np.asarray(u, dtype=np.float32), device=Z.device)
+        if u.shape != (Z.shape[0],):
+            raise ValueError(f"u must hold one number per row ({Z.shape[0]})")
+        kw = dict(temperature=float(temperature), top_k=int(top_k), top_p=float(top_p), min_p=float(min_p))
+        if not (kw["temperature"] >= 0 and kw["top_k"] >= 0 and 0 <= kw["top_p"] <= 1 and 0 <= kw["min_p"] <= 1):
+            raise ValueError(f"temperature and top_k must be >= 0, top_p and min_p in [0, 1] (got {kw})")
+        if Z.is_cuda:
+            from mlapi_amd.ops.logits import sample_logits
+
+            i, p = sample_logits(Z, u, **kw)
+        else:
+            from mlapi_amd.ops.reference import sample_ref
+
+            i, p = sample_ref(Z, u, **kw)
+        return self._m().classes[i.cpu().numpy()], p.float().cpu().numpy()
+
     def score(self, X, y) -> float:
         return float(np.mean(self.predict(X) == np.asarray(y)))
 

@@ -145,6 +145,16 @@ class LinearModel:
             s = 1.0 / (1.0 + np.exp(-z))  # OVR
             return s / s.sum(axis=1, keepdims=True)
 
+    def class_logits(self, X) -> np.ndarray:
+        """[n, n_classes] logits whose softmax is :meth:`predict_proba`, of every kind: z; [0, z] or [-z, z] of a binary
+        model; ln sigmoid(z) of a one-vs-rest one."""
+        z = self.decision_function(X)
+        if self.kind == Kind.BINARY:
+            return np.stack([np.zeros_like(z), z], axis=1)
+        if self.kind == Kind.BINARY_SOFTMAX:
+            return np.stack([-z, z], axis=1)
+        return z if self.kind == Kind.MULTINOMIAL else -np.logaddexp(0.0, -z)
+
     def predict_index(self, X) -> np.ndarray:
         z = self.decision_function(X)
         if self.n_outputs == 1:

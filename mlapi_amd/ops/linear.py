@@ -413,6 +413,67 @@ def softmax_train_grad(X_aug: torch.Tensor, W: torch.Tensor, b: torch.Tensor, y:
     return dW_out, stats
 
 
+def softmax_distill_grad(X_aug: torch.Tensor, W: torch.Tensor, b: torch.Tensor, idx: torch.Tensor, t: torch.Tensor, *,
+                         temperature: float = 1.0, alpha: float = 1.0, y: torch.Tensor = None,
+                         ws: torch.Tensor = None, dW_out: torch.Tensor = None, stats_out: torch.Tensor = None,
+                         update: dict = None, p2p=None, timeout_ms: int = 60000):
+    """Sums over the batch of the distillation loss's gradient, intercept included: :func:`softmax_train_grad` with a
+    teacher's top logits (``idx`` int32 [B, k], ``t`` [B, k]; :func:`mlapi_amd.ops.logits.top_logits`) as soft targets and
+    the labels ``y`` at weight 1 - alpha (:func:`mlapi_amd.ops.logits.distill_loss` has the formula). Returns
+    (dW_aug f32 [K, Fk + 8], stats f32 [loss_sum, n_correct]; n_correct is 0 without y). X_aug, W, b, ``update``
+    and ``p2p`` as there. ``ws``: a uint8 workspace of ``softmax_distill_workspace(B, K, Fk)`` bytes to keep."""
+    from mlapi_amd.ops.logits import _DT as _LOGIT_DT, MAX_TOP
+
+    _check(W, b)
+    for v in (X_aug, idx, t):
+        if not isinstance(v, torch.Tensor) or not v.is_cuda:
+            raise ValueError("mlapi_amd.ops: inputs must be GPU tensors (no CPU fallback)")
+    if X_aug.dtype != torch.bfloat16 or W.dtype != torch.bfloat16 or b.dtype != torch.float32:
+        raise TypeError("softmax_distill_grad: X_aug, W bf16 and b f32")
+    if idx.dtype != torch.int32 or t.dtype not in _LOGIT_DT:
+        raise TypeError("softmax_distill_grad: idx int32, t f32, bf16 or f16")
+    B, F_aug = X_aug.shape
+    K, F = W.shape
+    ldx = X_aug.stride(0) if B > 0 else F_aug
+    if X_aug.stride(1) != 1 or ldx < F_aug or ldx % 8 != 0:
+        raise ValueError("mlapi_amd.ops: X_aug rows must be contiguous with a row stride >= F_aug, a "
+                         "multiple of 8")
+    if gemm_width(F) != F or F_aug != F + 8 or b.numel() != K:
+        raise ValueError("softmax_distill_grad: shape mismatch (W must be [K, Fk], X_aug [B, Fk + 8])")
+    k = idx.shape[1] if idx.dim() == 2 else 0
+    if idx.shape != (B, k) or t.shape != (B, k) or not 1 <= k <= MAX_TOP or (k > 1 and (idx.stride(1), t.stride(1)) != (1, 1)):
+        raise ValueError(f"softmax_distill_grad: idx and t must be [B, k] with contiguous rows, 1 <= k <= {MAX_TOP}")
+    if y is not None and (not y.is_cuda or y.dtype != torch.int32 or y.shape != (B,) or not y.is_contiguous()):
+        raise ValueError("softmax_distill_grad: y must be a contiguous int32 [B] GPU tensor")
+    if alpha != 1.0 and y is None:
+        raise ValueError("softmax_distill_grad: alpha below 1 mixes in hard labels and needs y")
+    nbytes = C().softmax_distill_workspace(B, K, F)
+    if ws is None:
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=X_aug.device)
+    if stats_out is None:
+        stats_out = torch.zeros(2, dtype=torch.float32, device=X_aug.device)
+    if dW_out is None:
+        dW_out = torch.empty(K, F_aug, dtype=torch.float32, device=X_aug.device)
+    if not dW_out.is_contiguous() or dW_out.shape != (K, F_aug) or dW_out.dtype != torch.float32:
+        raise ValueError("softmax_distill_grad: dW_out must be a contiguous f32 [K, Fk + 8] tensor")
+    upd = {}
+    if update is not None:
+        p = update["params"]
+        if not p.is_contiguous() or p.shape != (K, F_aug) or p.dtype != torch.float32:
+            raise ValueError("softmax_distill_grad: update params must be a contiguous f32 [K, Fk + 8] tensor")
+        ptr = lambda v: 0 if v is None else v.data_ptr()  # noqa: E731
+        upd = dict(params=p.data_ptr(), mom=ptr(update.get("mom_buf")), shadow_w=ptr(update.get("shadow_w")),
+                   shadow_b=ptr(update.get("shadow_b")), pen_cols=F, lr=float(update["lr"]),
+                   inv_n=float(update["inv_n"]), l2=float(update.get("l2", 0.0)),
+                   momentum=float(update.get("momentum", 0.0)))
+    C().softmax_distill(X_aug.data_ptr(), ldx, W.data_ptr(), b.data_ptr(), idx.data_ptr(),
+                        idx.stride(0) if B > 1 else k, t.data_ptr(), t.stride(0) if B > 1 else k, _LOGIT_DT[t.dtype], k,
+                        float(temperature), float(alpha), 0 if y is None else y.data_ptr(), B, F, K, dW_out.data_ptr(),
+                        stats_out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(), **upd,
+                        p2p=None if p2p is None else p2p.native, timeout_ms=int(timeout_ms))
+    return dW_out, stats_out
+
+
 def sgd_update_2d(params: torch.Tensor, grad: torch.Tensor, pen_cols: int, lr: float, inv_n: float, l2: float,
                   momentum: float = 0.0, mom_buf: torch.Tensor = None, shadow_w: torch.Tensor = None,
                   shadow_b: torch.Tensor = None) -> None:

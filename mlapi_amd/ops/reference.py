@@ -167,3 +167,13 @@ def sample_ref(Z, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     prob = w.gather(1, idx[:, None])[:, 0] / mass[:, -1].clamp(min=1e-300)
     none = mass[:, -1] == 0
     return torch.where(none, -1, idx).to(torch.int32), torch.where(none, torch.zeros_like(prob), prob)
+
+
+def softmax_distill_ref(X_aug, W_aug, idx, t, *, temperature=1.0, alpha=1.0, y=None, dtype=torch.float32):
+    """Oracle of ops.linear.softmax_distill_grad: (G [B, K], dW_aug [K, F_aug], loss_sum, n_correct). Also the CPU path of
+    the trainer's distillation (dtype float32)."""
+    X = X_aug.to(dtype)
+    z = X @ W_aug.to(dtype).T
+    loss, G = distill_ref(z, idx, t, temperature=temperature, alpha=alpha, y=y, dtype=dtype)
+    correct = 0.0 if y is None else (torch.argmax(z, dim=1) == y.long()).sum().to(dtype)
+    return G, G.T @ X, loss.sum(), correct

@@ -12,7 +12,9 @@ LogisticRegression() (L-BFGS, C=1), pickle it to LRClassifier.pkl, reload it, pr
 runs data-parallel mini-batch SGD on synthetic data with checkpoint/resume
 in the native format (``--ckpt``; ``--resume``). ``--classes K`` (K > 2) trains a softmax
 (``--kind multinomial``) or one-vs-rest model with the MFMA gradient kernels; ``--graph``
-captures a single-GPU step in a HIP graph.
+captures a single-GPU step in a HIP graph. ``--teacher CKPT`` (a model of the same features and classes, native or
+sklearn format) distils instead: its ``--teacher-top`` largest logits per row are the targets, at
+``--temperature``, mixed with the labels at weight 1 - ``--alpha``.
 """
 from __future__ import annotations
 
@@ -115,7 +117,7 @@ def cmd_sgd_multiclass(args) -> int:
     from mlapi_amd.models.linear import Kind
     from mlapi_amd.parallel.comm import barrier, init_distributed, shutdown
     from mlapi_amd.train.schedule import BatchSchedule
-    from mlapi_amd.train.softmax_sgd import SoftmaxSGDTrainer, synthetic_multiclass
+    from mlapi_amd.train.softmax_sgd import SoftmaxSGDTrainer, synthetic_multiclass, teacher_top
 
     info = init_distributed()
     dev = info.device
@@ -123,8 +125,16 @@ def cmd_sgd_multiclass(args) -> int:
     X, y = synthetic_multiclass(args.rows_per_rank, args.features, args.classes, seed=1000 + info.rank,
                                 device=dev, noise=args.noise)
     tr = SoftmaxSGDTrainer(args.features, args.classes, kind=kind, info=info, lr=args.lr, l2=args.l2,
-                           momentum=args.momentum, device=dev)
+                           momentum=args.momentum, device=dev, temperature=args.temperature, alpha=args.alpha)
     Xa = tr.prepare(X)
+    top = None
+    if args.teacher:
+        from mlapi_amd.ckpt.native import load_model
+
+        teacher = load_model(args.teacher)
+        if teacher.n_outputs != args.classes:
+            raise SystemExit(f"--teacher has {teacher.n_outputs} classes, --classes is {args.classes}")
+        top = teacher_top(teacher, X, min(args.teacher_top, args.classes))
     del X
     nb = max(1, args.rows_per_rank // args.batch)
     sched = BatchSchedule(nb, seed=args.seed, shuffle=not args.no_shuffle)
@@ -138,7 +148,8 @@ def cmd_sgd_multiclass(args) -> int:
         sched.restore(st.epoch, st.data_cursor, st.rng_state)
         if info.is_main:
             print(f"resumed from {args.ckpt} at step {start} (epoch {st.epoch}, batch {st.data_cursor})", flush=True)
-    shards = [(Xa[j * args.batch:(j + 1) * args.batch], y[j * args.batch:(j + 1) * args.batch]) for j in range(nb)]
+    cut = lambda v, j: v[j * args.batch:(j + 1) * args.batch]  # noqa: E731
+    shards = [(cut(Xa, j), cut(y, j), None if top is None else (cut(top[0], j), cut(top[1], j))) for j in range(nb)]
     if args.graph and dev is not None and info.world == 1 and nb == 1:  # one batch: order is moot
         tr.capture(*shards[0])  # one HIP graph launch per step
     t0 = time.perf_counter()
@@ -199,6 +210,10 @@ def main(argv=None) -> int:
     p.add_argument("--kind", default="multinomial", choices=["multinomial", "ovr"])
     p.add_argument("--noise", type=float, default=1.0, help="multiclass synthetic label noise")
     p.add_argument("--graph", action="store_true", help="capture the single-GPU step in a HIP graph")
+    p.add_argument("--teacher", default="", help="checkpoint of the model to distil from (softmax, classes > 2)")
+    p.add_argument("--teacher-top", type=int, default=16, help="teacher logits kept per row")
+    p.add_argument("--temperature", type=float, default=2.0, help="of the distillation")
+    p.add_argument("--alpha", type=float, default=0.5, help="weight of the teacher's targets; 1 - alpha: the labels'")
     p.add_argument("--seed", type=int, default=0, help="mini-batch order (epoch shuffles; same on every rank)")
     p.add_argument("--no-shuffle", action="store_true", help="visit the batches in order every epoch")
     args = ap.parse_args(argv)

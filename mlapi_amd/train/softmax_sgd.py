@@ -19,6 +19,11 @@ This module is the scale-out counterpart (BASELINE config 5 with K classes): per
   hosts (or ``MLAPI_DP_FUSED=0``) fall back to an RCCL all-reduce of the fused buffer followed by
   ``sgd_update_2d``.
 
+With ``teacher=(idx, t)`` - a teacher's top logits of the batch's rows, :func:`teacher_top` - a step distils
+instead: the targets are the teacher's softmax over its list at the trainer's ``temperature``, mixed with the
+labels at weight 1 - ``alpha`` (:func:`mlapi_amd.ops.linear.softmax_distill_grad`; the update and the exchange are the
+same).
+
 fp32 master weights; every rank applies the identical update, so replicas stay bitwise equal.
 One replica (world == 1) can capture the whole step in a HIP graph (:meth:`capture`).
 """
@@ -43,6 +48,32 @@ def synthetic_multiclass(n: int, F: int, K: int, *, seed: int = 0, device=None, 
     return X.to(device), y.to(device)
 
 
+def teacher_top(model, X: torch.Tensor, k: int, *, rows: int = 1 << 16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What a teacher (a :class:`~mlapi_amd.models.linear.LinearModel` of at least 3 classes) writes down for the rows of
+    X [n, F]: the classes (int32 [n, k]) and logits (f32 [n, k]) of its k largest logits, on X's device. On a GPU its
+    logits are bf16 products with f32 sums, ``rows`` rows at a time."""
+    W, b = torch.as_tensor(model.W), torch.as_tensor(model.b)
+    if W.shape[0] < 2 or W.shape[1] != X.shape[1]:
+        raise ValueError(f"the teacher must have one row per class and {X.shape[1]} features (W is {tuple(W.shape)})")
+    if not 1 <= k <= W.shape[0]:
+        raise ValueError(f"the teacher has {W.shape[0]} classes: k must be in [1, {W.shape[0]}] (got {k})")
+    if not X.is_cuda:
+        from mlapi_amd.ops.reference import top_logits_ref
+
+        t, idx = top_logits_ref((X.double() @ W.T + b).float(), k)
+        return idx, t
+    from mlapi_amd.ops.linear import gemm_logits
+    from mlapi_amd.ops.logits import top_logits
+
+    idx = torch.empty(X.shape[0], k, dtype=torch.int32, device=X.device)
+    t = torch.empty(X.shape[0], k, dtype=torch.float32, device=X.device)
+    W, b = W.to(X.device, torch.bfloat16), b.to(X.device, torch.float32)
+    for s in range(0, X.shape[0], rows):
+        Z = gemm_logits(X[s:s + rows].to(torch.bfloat16).contiguous(), W, b)
+        top_logits(Z, k, out=(t[s:s + rows], idx[s:s + rows]))
+    return idx, t
+
+
 def _kernel_width(F: int) -> int:
     from mlapi_amd.ops.linear import softmax_kernel_width
 
@@ -54,7 +85,9 @@ class SoftmaxSGDTrainer:
 
     def __init__(self, n_features: int, n_classes: int, *, kind: int = Kind.MULTINOMIAL,
                  info: Optional[DistInfo] = None, lr: float = 0.1, l2: float = 0.0, momentum: float = 0.0,
-                 device=None):
+                 device=None, temperature: float = 1.0, alpha: float = 1.0):
+        if not (1e-6 <= temperature <= 1e6 and 0.0 <= alpha <= 1.0):
+            raise ValueError("SoftmaxSGDTrainer: temperature must be in [1e-6, 1e6] and alpha in [0, 1]")
         if kind not in (Kind.MULTINOMIAL, Kind.OVR):
             raise ValueError("SoftmaxSGDTrainer: kind must be MULTINOMIAL or OVR (binary: BinarySGDTrainer)")
         if n_classes < 2:
@@ -68,6 +101,7 @@ class SoftmaxSGDTrainer:
             self.device = torch.device("cpu")
         self.on_gpu = torch.device(self.device).type == "cuda"
         self.lr, self.l2, self.momentum = lr, l2, momentum
+        self.temperature, self.alpha = float(temperature), float(alpha)  # of steps with a teacher
         self.params = torch.zeros(self.K, self.F_aug, dtype=torch.float32, device=self.device)
         # what the MFMA forward reads: bf16 W [K, Fk] and f32 intercepts (refreshed by every update)
         self.shadow_w = torch.zeros(self.K, self.Fk, dtype=torch.bfloat16, device=self.device) if self.on_gpu else None
@@ -76,6 +110,7 @@ class SoftmaxSGDTrainer:
         self.grad = torch.zeros(n + 2, dtype=torch.float32, device=self.device)  # [dW_aug | loss | correct]
         self.mom = torch.zeros_like(self.params) if momentum else None
         self._bufs = {}  # batch size -> SoftmaxTrainBuffers (a ragged last batch keeps its own)
+        self._distill_ws = {}  # batch size -> workspace of its distillation steps
         self._graph = None
         self._dp = None
         if self.on_gpu:
@@ -158,7 +193,7 @@ class SoftmaxSGDTrainer:
         self._refresh_shadow()
         return False
 
-    def _local_grad(self, Xa: torch.Tensor, y: torch.Tensor, fused_update_n: int = 0, dp=None) -> None:
+    def _local_grad(self, Xa: torch.Tensor, y: torch.Tensor, fused_update_n: int = 0, dp=None, teacher=None) -> None:
         """Gradient sums into self.grad; with ``fused_update_n`` the SGD update for that global
         batch size runs inside the gradient's final slab sum, after the in-kernel DP exchange when
         ``dp`` is given (then self.grad holds the global sums)."""
@@ -166,22 +201,42 @@ class SoftmaxSGDTrainer:
             from mlapi_amd.ops.linear import SoftmaxTrainBuffers, softmax_train_grad
 
             B = Xa.shape[0]
-            if B not in self._bufs:
-                self._bufs[B] = SoftmaxTrainBuffers(B, self.K, self.Fk, Xa.device)
             upd = None
             if fused_update_n:
                 upd = dict(params=self.params, lr=self.lr, inv_n=1.0 / fused_update_n, l2=self.l2,
                            momentum=self.momentum, mom_buf=self.mom, shadow_w=self.shadow_w, shadow_b=self.shadow_b)
+            if teacher is not None:
+                self._distill_grad(Xa, y, teacher, upd, dp)
+                return
+            if B not in self._bufs:
+                self._bufs[B] = SoftmaxTrainBuffers(B, self.K, self.Fk, Xa.device)
             softmax_train_grad(Xa, self.shadow_w, self.shadow_b, y, self.kind, bufs=self._bufs[B], dW_out=self._dW(),
                                stats_out=self.grad[self.K * self.F_aug:], update=upd, p2p=dp,
                                timeout_ms=self.dp_timeout_ms)
         else:
-            from mlapi_amd.ops.reference import softmax_train_ref
+            from mlapi_amd.ops.reference import softmax_distill_ref, softmax_train_ref
 
-            _, dW, loss, correct = softmax_train_ref(Xa, y, self.params, self.kind)
+            if teacher is not None:
+                _, dW, loss, correct = softmax_distill_ref(Xa, self.params, *teacher, temperature=self.temperature,
+                                                           alpha=self.alpha, y=y)
+            else:
+                _, dW, loss, correct = softmax_train_ref(Xa, y, self.params, self.kind)
             self._dW().copy_(dW)
             self.grad[-2] = loss
             self.grad[-1] = correct
+
+    def _distill_grad(self, Xa, y, teacher, upd, dp) -> None:
+        from mlapi_amd._native import C
+        from mlapi_amd.ops.linear import softmax_distill_grad
+
+        B = Xa.shape[0]
+        if B not in self._distill_ws:
+            self._distill_ws[B] = torch.empty(max(16, C().softmax_distill_workspace(B, self.K, self.Fk)),
+                                              dtype=torch.uint8, device=Xa.device)
+        softmax_distill_grad(Xa, self.shadow_w, self.shadow_b, *teacher, temperature=self.temperature, alpha=self.alpha,
+                             y=y, ws=self._distill_ws[B], dW_out=self._dW(),
+                             stats_out=self.grad[self.K * self.F_aug:], update=upd, p2p=dp,
+                             timeout_ms=self.dp_timeout_ms)
 
     def _update(self, n_global: int) -> None:
         if self.on_gpu:
@@ -197,45 +252,52 @@ class SoftmaxSGDTrainer:
                 d = self.mom
             self.params.sub_(self.lr * d)
 
-    def step(self, Xa: torch.Tensor, y: torch.Tensor) -> None:
-        """One SGD step on this rank's shard (Xa from :meth:`prepare`, y int32 class indices)."""
-        if self._graph is not None and self._graph[1] is Xa and self._graph[2] is y:
+    def _check_teacher(self, teacher) -> None:
+        if teacher is not None and self.kind != Kind.MULTINOMIAL:
+            raise ValueError("SoftmaxSGDTrainer: distillation is for softmax (MULTINOMIAL) models")
+
+    def step(self, Xa: torch.Tensor, y: torch.Tensor, teacher=None) -> None:
+        """One SGD step on this rank's shard (Xa from :meth:`prepare`, y int32 class indices). ``teacher``: (idx, t) of
+        the same rows (:func:`teacher_top`) makes it a distillation step; y may then be None at alpha 1."""
+        self._check_teacher(teacher)
+        if self._graph is not None and self._graph[1] is Xa and self._graph[2] is y and self._graph[3] is teacher:
             self._graph[0].replay()
         elif self.on_gpu and (self._dp is not None or self.info.world == 1):
-            self._local_grad(Xa, y, fused_update_n=Xa.shape[0] * self.info.world, dp=self._dp)
+            self._local_grad(Xa, y, fused_update_n=Xa.shape[0] * self.info.world, dp=self._dp, teacher=teacher)
             if self._dp is not None:
                 self._dp.check_now()  # a missed exchange stops the loop (ADVICE r3: no silent divergence)
                 if self.verify_every > 0 and (self.steps + 1) % self.verify_every == 0:
                     self.verify_replicas()
         else:
-            self._local_grad(Xa, y)
+            self._local_grad(Xa, y, teacher=teacher)
             all_reduce_sum_(self.grad, self.info)
             self._update(Xa.shape[0] * self.info.world)
         self.steps += 1
         self._n_seen = Xa.shape[0] * self.info.world
 
-    def capture(self, Xa: torch.Tensor, y: torch.Tensor) -> None:
+    def capture(self, Xa: torch.Tensor, y: torch.Tensor, teacher=None) -> None:
         """Capture one whole step (row stats + fused gradient + slab sums + update) in a HIP graph.
 
-        Later ``step(Xa, y)`` calls with these exact tensors replay it: one launch from the host.
+        Later ``step(Xa, y, teacher)`` calls with these exact objects replay it: one launch from the host.
         Single replica only (the all-reduce stays outside graphs)."""
         if not self.on_gpu or self.info.world != 1:
             raise RuntimeError("graph capture: single-GPU replica only")
+        self._check_teacher(teacher)
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         saved = (self.params.clone(), None if self.mom is None else self.mom.clone())
         with torch.cuda.stream(s):  # warm-up: allocates the buffers
             for _ in range(2):
-                self._local_grad(Xa, y, fused_update_n=Xa.shape[0], dp=self._dp)
+                self._local_grad(Xa, y, fused_update_n=Xa.shape[0], dp=self._dp, teacher=teacher)
         torch.cuda.current_stream().wait_stream(s)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            self._local_grad(Xa, y, fused_update_n=Xa.shape[0], dp=self._dp)
+            self._local_grad(Xa, y, fused_update_n=Xa.shape[0], dp=self._dp, teacher=teacher)
         self.params.copy_(saved[0])
         self._refresh_shadow()
         if self.mom is not None:
             self.mom.copy_(saved[1])
-        self._graph = (g, Xa, y)
+        self._graph = (g, Xa, y, teacher)
 
     # ---------------------------------------------------------------------------------- stats
     def last_loss(self) -> float:

@@ -1,0 +1,241 @@
+"""Distillation through the trainer, the CLI and the estimator: a teacher's top logits, the student's steps, its answers."""
+import json
+import subprocess
+import sys
+from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+
+from logits_cases import INF, rows
+from mlapi_amd.models.estimator import LogisticRegression
+from mlapi_amd.models.linear import Kind, LinearModel
+from mlapi_amd.ops import reference as ref
+from mlapi_amd.train.softmax_sgd import SoftmaxSGDTrainer, synthetic_multiclass, teacher_top
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+def test_cpu_step_follows_the_formula():
+    n, F, K, k, T, alpha, lr, l2 = 40, 9, 6, 3, 2.0, 0.3, 0.5, 1e-2
+    X, y = synthetic_multiclass(n, F, K, seed=1)
+    idx, t = teacher_top(LinearModel.random(F, K, seed=5), X, k)
+    tr = SoftmaxSGDTrainer(F, K, lr=lr, l2=l2, device=torch.device("cpu"), temperature=T, alpha=alpha)
+    W0, b0 = torch.randn(K, F), torch.randn(K)
+    tr.set_params(W0, b0)
+    W, b = W0.double().requires_grad_(), b0.double().requires_grad_()
+    z = X.to(torch.bfloat16).double() @ W.T + b  # features are prepared in bf16 on both devices
+    q = torch.softmax(t.double() / T, 1)
+    soft = (q * (q.log() - torch.log_softmax(z / T, 1).gather(1, idx.long()))).sum(1)
+    loss = (alpha * T * T * soft - (1 - alpha) * torch.log_softmax(z, 1)[torch.arange(n), y.long()]).sum()
+    loss.backward()
+    tr.step(tr.prepare(X), y, teacher=(idx, t))
+    # f32 sums over n rows of terms below 8: 64 roundings of 2^-24 are ample
+    tol = 64 * 2.0 ** -24 * n * 8
+    assert (tr.W - (W0 - lr * (W.grad / n + l2 * W0))).abs().max() <= tol
+    assert (tr.b - (b0 - lr * b.grad / n)).abs().max() <= tol
+    assert abs(tr.last_loss() - loss.item() / n) <= tol
+    assert tr.last_accuracy() == (z.argmax(1) == y).double().mean().item()
+
+
+def test_trainer_refusals():
+    X, y = synthetic_multiclass(8, 4, 3)
+    idx, t = teacher_top(LinearModel.random(4, 3, seed=0), X, 2)
+    ovr = SoftmaxSGDTrainer(4, 3, kind=Kind.OVR, device=torch.device("cpu"))
+    with pytest.raises(ValueError, match="softmax"):
+        ovr.step(ovr.prepare(X), y, teacher=(idx, t))
+    for kw in (dict(temperature=0.0), dict(alpha=1.1)):
+        with pytest.raises(ValueError):
+            SoftmaxSGDTrainer(4, 3, device=torch.device("cpu"), **kw)
+    with pytest.raises(ValueError, match="features"):
+        teacher_top(LinearModel.random(5, 3, seed=0), X, 2)
+    with pytest.raises(ValueError, match="k must be"):
+        teacher_top(LinearModel.random(4, 3, seed=0), X, 4)
+
+
+def test_teacher_of_all_classes_and_temperature_one_gives_its_own_weights_no_gradient():
+    """A student that equals its teacher has nothing to learn but what preparing the features in bf16 moved."""
+    X, y = synthetic_multiclass(30, 6, 5, seed=2)
+    m = LinearModel.random(6, 5, seed=1)
+    tr = SoftmaxSGDTrainer(6, 5, lr=1.0, device=torch.device("cpu"))
+    tr.set_params(torch.as_tensor(m.W), torch.as_tensor(m.b))
+    before = tr.params.clone()
+    tr.step(tr.prepare(X), y, teacher=teacher_top(m, X, 5))
+    # a row's logits move by d = W (X - bf16(X)), p by at most 2 max |d|, and KL(q || p) <= 2 max |d|; the
+    # gradient is the mean of p - q times the features. f32: logits below 16 are 2^-20 off, features below 4
+    d = ((X - X.to(torch.bfloat16).float()).double() @ torch.as_tensor(m.W).T).abs().amax(1)
+    reach = torch.cat([X.abs().double(), torch.ones(30, 1)], 1).amax(1)
+    assert (tr.params - before).abs().max() <= (2 * d * reach).mean() + 4 * 2.0 ** -18
+    assert abs(tr.last_loss()) <= (2 * d).mean() + 2.0 ** -18
+
+
+def _cli(*args):
+    r = subprocess.run([sys.executable, "-m", "mlapi_amd.train", "sgd", *args], capture_output=True, text=True, cwd=ROOT,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return json.loads(r.stdout.strip().splitlines()[-1])
+
+
+def test_cli_distils_from_a_checkpoint(tmp_path):
+    from mlapi_amd.ckpt.native import save_native
+
+    path = str(tmp_path / "teacher.safetensors")
+    save_native(path, LinearModel.random(12, 5, seed=3))
+    out = _cli("--features", "12", "--classes", "5", "--rows-per-rank", "256", "--batch", "64", "--steps", "6", "--teacher",
+               path, "--teacher-top", "3", "--alpha", "0.7")
+    assert out["classes"] == 5 and np.isfinite(out["final_loss"])
+
+
+# ---------------------------------------------------------------------------------------- answers
+@pytest.fixture(scope="module")
+def estimator():
+    clf = LogisticRegression(device="cpu")
+    clf.model_ = LinearModel.random(7, 6, seed=4, labels=list("abcdef"))
+    return clf
+
+
+def test_class_logits_give_predict_proba_for_every_kind():
+    rng = np.random.default_rng(0)
+    X = rng.standard_normal((20, 4))
+    for kind, K in ((Kind.BINARY, 2), (Kind.BINARY_SOFTMAX, 2), (Kind.MULTINOMIAL, 5), (Kind.OVR, 5)):
+        m = LinearModel.random(4, K, seed=1, kind=kind)
+        z = m.class_logits(X)
+        e = np.exp(z - z.max(1, keepdims=True))
+        np.testing.assert_allclose(e / e.sum(1, keepdims=True), m.predict_proba(X), rtol=1e-12, atol=1e-15)
+
+
+def test_estimator_samples_and_tops(estimator):
+    X = np.random.default_rng(1).standard_normal((50, 7))
+    label, prob = estimator.sample(X, temperature=0.0)
+    assert (label == estimator.predict(X)).all() and (prob == 1).all()
+    top, z = estimator.predict_top(X, 3)
+    assert (top[:, 0] == estimator.predict(X)).all() and (np.diff(z, axis=1) <= 0).all()
+    label, prob = estimator.sample(X, np.full(50, 0.5), top_k=1)
+    assert (label == top[:, 0]).all() and (prob == 1).all()
+    label, prob = estimator.sample(X, np.zeros(50), top_p=1.0)  # the first class of all
+    assert (label == "a").all()
+    np.testing.assert_allclose(prob, estimator.predict_proba(X)[:, 0], rtol=1e-5)
+    with pytest.raises(ValueError):
+        estimator.sample(X, np.zeros(3))
+    with pytest.raises(ValueError):
+        estimator.sample(X, top_p=1.5)
+    with pytest.raises(ValueError):
+        estimator.predict_top(X, 7)
+
+
+@pytest.mark.gpu
+def test_estimator_on_the_gpu_answers_as_on_the_cpu(estimator):
+    X = np.random.default_rng(2).standard_normal((300, 7))
+    u = np.random.default_rng(3).random(300)
+    gpu = LogisticRegression(device="cuda")
+    gpu.model_ = estimator.model_
+    for kw in (dict(), dict(temperature=0.5, top_p=0.8), dict(top_k=3, min_p=0.1)):
+        a, b = estimator.sample(X, u, **kw), gpu.sample(X, u, **kw)
+        assert (a[0] == b[0]).all()
+        np.testing.assert_allclose(a[1], b[1], rtol=2.0 ** -22)
+    a, b = estimator.predict_top(X, 4), gpu.predict_top(X, 4)
+    assert (a[0] == b[0]).all() and (a[1] == b[1]).all()
+
+
+# ------------------------------------------------------------------------------------- on the GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,F,K,k", [(1, 128, 2, 1), (70, 128, 40, 5), (300, 256, 1000, 16), (1111, 512, 77, 77),
+                                     (513, 768, 130, 9), (64, 256, 2100, 33)])
+@pytest.mark.parametrize("alpha", [1.0, 0.4])
+def test_gradient_against_the_plain_form(B, F, K, k, alpha):
+    from mlapi_amd.ops import linear as ops
+
+    dev, T = "cuda:0", 2.0
+    g = torch.Generator().manual_seed(B + K)
+    X = torch.randn(B, F, generator=g).to(dev)
+    Xa = ops.augment_features(X, F + 8)
+    W = (torch.randn(K, F, generator=g) / F ** 0.5).to(torch.bfloat16).to(dev)
+    b = (0.1 * torch.randn(K, generator=g)).to(dev)
+    y = torch.randint(0, K, (B,), generator=g).to(torch.int32).to(dev)
+    idx, t = teacher_top(LinearModel(W.double().cpu().numpy() * 1.3, np.zeros(K), np.arange(K), Kind.MULTINOMIAL), X, k)
+    idx[0, 0] = -1  # a short list
+    dW, stats = ops.softmax_distill_grad(Xa, W, b, idx, t, temperature=T, alpha=alpha, y=y)
+    Wa = torch.cat([W.double(), b.double()[:, None], torch.zeros(K, 7, device=dev, dtype=torch.float64)], 1)
+    G, rdW, loss, correct = ref.softmax_distill_ref(Xa, Wa, idx, t, temperature=T, alpha=alpha, y=y, dtype=torch.float64)
+    # logits: F + 1 products summed in f32; G moves by at most twice that (both softmaxes have slope at most
+    # 1), by the 1000 roundings of a row's f32 sums, and by its rounding to bf16; then a sum over B rows in f32
+    u = 2.0 ** -24
+    ez = (F + 2) * u * (Xa.double().abs() @ Wa.abs().T).max()
+    eG = G.abs() * 2.0 ** -8 + 2 * ez + 1000 * u * T
+    tol = eG.T @ Xa.double().abs() + (B + 64) * u * (G.abs().T @ Xa.double().abs())
+    assert ((dW.double() - rdW).abs() <= tol + 1e-30).all(), ((dW.double() - rdW).abs() - tol).max()
+    assert abs(stats[0].item() - loss.item()) <= B * (T * T * (2 * ez.item() + 1000 * u) * 4) + abs(loss.item()) * 1000 * u
+    z = (Xa.double() @ Wa.T)
+    top = torch.topk(z, 2, dim=1).values
+    sure = (top[:, 0] - top[:, 1]) > 2 * ez  # rows whose maximum rounding cannot move
+    assert abs(stats[1].item() - correct.item()) <= (~sure).sum().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("momentum", [0.0, 0.9])
+def test_trainer_steps_on_the_gpu_follow_the_cpu_ones_and_a_captured_step_the_eager_one(momentum):
+    dev = torch.device("cuda", 0)
+    n, F, K, k = 640, 60, 23, 6
+    X, y = synthetic_multiclass(n, F, K, seed=3)
+    m = LinearModel.random(F, K, seed=9)
+    kw = dict(lr=0.3, l2=1e-3, momentum=momentum, temperature=1.5, alpha=0.5)
+    cpu, gpu, graphed = (SoftmaxSGDTrainer(F, K, device=d, **kw) for d in (torch.device("cpu"), dev, dev))
+    top = teacher_top(m, X.to(torch.bfloat16).float(), k)
+    on = tuple(v.to(dev) for v in top)
+    Xc, Xg, yg = cpu.prepare(X.to(torch.bfloat16).float()), gpu.prepare(X.to(dev)), y.to(dev)
+    graphed.capture(Xg, yg, on)
+    for s in range(4):
+        cpu.step(Xc, y, teacher=top)
+        gpu.step(Xg, yg, teacher=on)
+        graphed.step(Xg, yg, teacher=on)
+        torch.cuda.synchronize()
+        assert torch.equal(gpu.params, graphed.params) and gpu.last_loss() == graphed.last_loss()
+    # bf16 weights and gradients: 2^-8 of weights below 1 move a logit of 60 features by less than 2^-8 * 60^0.5 * 3,
+    # and every step's update of the mean gradient by as much times lr; momentum sums up to 10 of them
+    assert (cpu.W - gpu.W.cpu()).abs().max() <= 4 * 0.3 * (10 if momentum else 1) * 2.0 ** -8 * 24
+    assert torch.isfinite(gpu.params).all()
+
+
+@pytest.mark.gpu
+def test_teacher_student_answer_run():
+    """The run as it is used: the teacher's top logits, the student's steps, its drawn answers."""
+    dev = torch.device("cuda", 0)
+    n, F, K, k = 4096, 64, 40, 8
+    X, _ = synthetic_multiclass(n, F, K, seed=4, device=dev)
+    m = LinearModel.random(F, K, seed=6, scale=3.0)
+    top = teacher_top(m, X, k)
+    student = SoftmaxSGDTrainer(F, K, lr=1.0, momentum=0.9, device=dev, temperature=2.0, alpha=1.0)
+    Xa = student.prepare(X)
+    for _ in range(20):
+        student.step(Xa, None, teacher=top)
+    clf = LogisticRegression(device="cuda")
+    clf.model_ = student.to_model()
+    label, prob = clf.sample(X.cpu().numpy(), top_k=5, temperature=0.7)
+    assert label.shape == (n,) and (prob > 0).all() and (prob <= 1).all()
+    tops, _ = clf.predict_top(X.cpu().numpy(), 5)
+    assert (tops == label[:, None]).any(1).all()
+
+
+@pytest.mark.gpu
+def test_distill_grad_refusals():
+    from mlapi_amd.ops import linear as ops
+
+    dev = "cuda:0"
+    Xa = ops.augment_features(torch.zeros(4, 128, device=dev), 136)
+    W, b = torch.zeros(5, 128, dtype=torch.bfloat16, device=dev), torch.zeros(5, device=dev)
+    idx, t = torch.zeros(4, 2, dtype=torch.int32, device=dev), torch.zeros(4, 2, device=dev)
+    ops.softmax_distill_grad(Xa, W, b, idx, t)
+    for kw in (dict(alpha=0.5), dict(temperature=0.0), dict(alpha=2.0), dict(y=idx[:, 0]),
+               dict(ws=torch.zeros(16, dtype=torch.uint8, device=dev))):
+        with pytest.raises(ValueError):
+            ops.softmax_distill_grad(Xa, W, b, idx, t, **kw)
+    for bad in ((Xa, W, b, idx[:3], t), (Xa, W, b, idx, t[:, :1]), (Xa, W[:, :100], b, idx, t), (Xa.cpu(), W, b, idx, t)):
+        with pytest.raises(ValueError):
+            ops.softmax_distill_grad(*bad)
+    with pytest.raises(TypeError):
+        ops.softmax_distill_grad(Xa, W, b, idx.long(), t)
+
+
+def test_rows_helper_masks():
+    assert (rows(2, 8, torch.float32, 0, "masked")[0] == -INF).all()
