@@ -54,18 +54,21 @@ struct Args {
   float T, soft, hard;  // soft = a, hard = 1 - a (0 without labels)
 };
 
-// The listed classes of one row, in LDS: n = k entries, and the label as one more.
+// The listed classes of one row, in LDS: n = k entries, and the label as one more; 14 bytes each, so
+// that four rows of 1024 entries stay below 64 KB.
 struct Listed {
-  int* cls;     // class, -1: absent
-  float* lq;    // log2 q_j
-  float* z;     // its logit
+  int* cls;        // class, -1: absent
+  float* lq;       // log2 q_j
+  float* z;        // its logit; later the whole gradient of the class
+  uint16_t* keep;  // whether this entry writes it
   __device__ Listed(unsigned char* lds, int cap) {
     cls = reinterpret_cast<int*>(lds);
     lq = reinterpret_cast<float*>(cls + cap);
     z = lq + cap;
+    keep = reinterpret_cast<uint16_t*>(z + cap);
   }
-  static __host__ __device__ int capacity(int k) { return (k + 1 + 3) / 4 * 4; }
-  static __host__ __device__ size_t bytes(int k) { return (size_t)capacity(k) * 12; }
+  static __host__ __device__ int capacity(int k) { return (k + 1 + 7) / 8 * 8; }
+  static __host__ __device__ size_t bytes(int k) { return (size_t)capacity(k) * 14; }
 };
 
 // Reads the row's entries (one wave): log2 q into lq (-inf: absent), logits into z. Returns Q (1, or 0 without entries; NaN
@@ -149,17 +152,17 @@ __device__ __forceinline__ void dense_coeffs(const Args& a, float g, float Q, fl
   a1 = none || H == 0.f ? 0.f : g * H / r.s1;
 }
 
-// Whole gradients of the listed classes in [c0, c1), into `out`; classes that another entry writes, or
-// that lie outside, become -1 in `keep`. One wave; L.cls is only read.
+// Whole gradients of the listed classes in [c0, c1), in the place of their logits; entries whose class
+// another entry writes, or that lie outside, are not kept. One wave.
 __device__ void listed_grads(const Args& a, int lane, Listed L, float g, float at, float a1, float m, float H,
-                             bool none, int c0, int c1, float* out, int* keep) {
+                             bool none, int c0, int c1) {
   const float ct = 1.44269504088896340736f / a.T, c1e = 1.44269504088896340736f;
   const int cap = Listed::capacity(a.k);
   for (int j = lane; j <= a.k; j += 64) {
     const int c = L.cls[j];
-    int mine = c >= c0 && c < c1 ? c : -1;
+    bool mine = c >= c0 && c < c1;
     float v = 0.f;
-    if (mine >= 0) {
+    if (mine) {
       float sum = 0.f;
       for (int i = 0; i < cap; i += 4) {
         const int4 o = *reinterpret_cast<const int4*>(L.cls + i);
@@ -167,7 +170,7 @@ __device__ void listed_grads(const Args& a, int lane, Listed L, float g, float a
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (oc[e] == c) {
-            if (i + e < j) mine = -1;
+            if (i + e < j) mine = false;
             sum += i + e == a.k ? H : a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[i + e]);
           }
       }
@@ -175,8 +178,8 @@ __device__ void listed_grads(const Args& a, int lane, Listed L, float g, float a
       v = none ? at : at * __builtin_amdgcn_exp2f(d * ct) - g * sum;
       if (!none && H != 0.f) v += a1 * __builtin_amdgcn_exp2f(d * c1e);
     }
-    out[j] = v;
-    keep[j] = mine;
+    L.z[j] = v;
+    L.keep[j] = mine ? 1 : 0;
   }
 }
 
@@ -193,10 +196,7 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
   const int64_t row = (int64_t)blockIdx.x * RPB + sub;
   if (row >= a.B) return;  // whole waves: rows of fewer than a block's threads have one wave, and no barrier
   const int K = a.K, cap = Listed::capacity(a.k);
-  unsigned char* mine = dyn + (size_t)sub * (cap * 20);
-  Listed L(mine, cap);
-  float* gv = reinterpret_cast<float*>(mine + cap * 12);
-  int* gc = reinterpret_cast<int*>(gv + cap);
+  Listed L(dyn + (size_t)sub * Listed::bytes(a.k), cap);
   const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
   Held<T> raw[NV];
   load_row<T, NTR, NV>(raw, z, tid, K);
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
       if (a.stats_out != nullptr) a.stats_out[row] = r;
       if (a.pred != nullptr) a.pred[row] = r.arg;
     }
-    if (a.dz != nullptr) listed_grads(a, lane, L, g, at, a1, m, H, r.st == 0.f, 0, K, gv, gc);
+    if (a.dz != nullptr) listed_grads(a, lane, L, g, at, a1, m, H, r.st == 0.f, 0, K);
   }
   again();
   TO* dz = static_cast<TO*>(a.dz) + row * a.ldd;
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
   if (a.dz == nullptr) return;
   sync();
   for (int j = tid; j <= a.k; j += NTR)
-    if (gc[j] >= 0) dz[gc[j]] = (TO)gv[j];
+    if (L.keep[j] != 0) dz[L.cls[j]] = (TO)L.z[j];
 }
 
 // ---- rows cut into parts ------------------------------------------------------------------------
@@ -453,8 +453,6 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
   const int lane = threadIdx.x & 63, cap = Listed::capacity(a.k);
   const float ct = 1.44269504088896340736f / a.T, ce = 1.44269504088896340736f;
   Listed L(dyn, cap);
-  float* gv = reinterpret_cast<float*>(dyn + cap * 12);
-  int* gc = reinterpret_cast<int*>(gv + cap);
   RowStats r = lane < a.parts ? a.stats_in[row * a.parts + lane] : RowStats{-__builtin_inff(), 0.f, 0.f, a.K};
   if (a.parts > 1) {
 #pragma unroll
@@ -485,7 +483,7 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
         if (a.pred != nullptr) a.pred[row] = r.arg;
       }
     }
-    if (a.dz != nullptr) listed_grads(a, lane, L, g, at, a1, m, H, r.st == 0.f, c0, c1, gv, gc);
+    if (a.dz != nullptr) listed_grads(a, lane, L, g, at, a1, m, H, r.st == 0.f, c0, c1);
   }
   if (a.dz == nullptr) return;
   __syncthreads();
@@ -496,14 +494,14 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
   stream_grad<T, TO, PART_THREADS>(a, z, dz, c0, c1, r, at, a1);
   __syncthreads();
   for (int j = threadIdx.x; j <= a.k; j += PART_THREADS)
-    if (gc[j] >= 0) dz[gc[j]] = (TO)gv[j];
+    if (L.keep[j] != 0) dz[L.cls[j]] = (TO)L.z[j];
 }
 
 // ---- host ---------------------------------------------------------------------------------------
 template <class T, class TO, int NTR, int NV>
 void launch_rows(const Args& a, hipStream_t stream) {
   constexpr int NT = NTR < 256 ? 256 : NTR, RPB = NT / NTR;
-  const size_t lds = (size_t)RPB * Listed::capacity(a.k) * 20;
+  const size_t lds = RPB * Listed::bytes(a.k);
   hipLaunchKernelGGL((distill_rows_kernel<T, TO, NTR, NV>), dim3((unsigned)((a.B + RPB - 1) / RPB)), dim3(NT), lds,
                      stream, a);
   MLAPI_HIP_CHECK(hipGetLastError());
@@ -555,7 +553,7 @@ template <class T, class TO>
 void run_distill(Args a, RowStats* ws, hipStream_t stream) {
   const Plan p = make_plan<T>(a.B, a.K);
   if (p.parts == 0) return launch_resident<T, TO>(a, stream);
-  const size_t lds = (size_t)Listed::capacity(a.k) * 20;
+  const size_t lds = Listed::bytes(a.k);
   a.parts = 1;
   for (int64_t r0 = 0; r0 < a.B; r0 += 65535) {  // grid.y holds 16 bits
     Args b = a;
@@ -601,6 +599,7 @@ void launch_distill(const DistillCall& c, hipStream_t stream) {
   if (c.B <= 0) return;
   if (c.K < 1 || c.K > LOGIT_MAX_CLASSES || c.k < 1 || c.k > LOGIT_MAX_TOP)
     throw std::invalid_argument("distill: 1 <= K <= 2^20 classes, 1 <= k <= 1024 entries");
+  if (c.B > 0x7fffffff) throw std::invalid_argument("distill: more than 2^31 rows");
   if (!(c.temperature >= 1e-6f && c.temperature <= 1e6f))
     throw std::invalid_argument("distill: temperature in [1e-6, 1e6]");
   if (!(c.alpha >= 0.f && c.alpha <= 1.f)) throw std::invalid_argument("distill: alpha in [0, 1]");

@@ -8,7 +8,8 @@
 //          first always (p >= 1: all);
 //   min-p: of those, the ones with w >= min_p (the largest has w = 1; min_p <= 0: all).
 // The draw is the first class, in class order, whose cumulative kept mass exceeds u times the kept
-// mass, u clamped into [0, 1); prob is its share of the kept mass. T <= 0 (or NaN) takes the first maximum.
+// mass, u clamped into [0, 1); prob is its share of the kept mass. T <= 0 takes the first maximum; T = inf or NaN counts as the
+// largest finite number.
 // Masked classes (-inf, NaN) are never drawn; a row without any other gives class -1, prob 0.
 //
 // Masses are integer sums of fixed-point weights (logit_rows.h), so a draw does not depend on how the
@@ -40,7 +41,8 @@ struct Settings {
 
 __device__ __forceinline__ Settings settings(const SampleCall& a, int64_t row) {
   Settings s;
-  s.T = a.temperature != nullptr ? a.temperature[row] : a.temperature_all;
+  // finite: an infinite temperature times an infinite difference, a masked class's, is no number
+  s.T = fminf(a.temperature != nullptr ? a.temperature[row] : a.temperature_all, 0x1.fffffep127f);
   s.top_p = a.top_p != nullptr ? a.top_p[row] : a.top_p_all;
   s.min_p = a.min_p != nullptr ? a.min_p[row] : a.min_p_all;
   s.top_k = a.top_k != nullptr ? a.top_k[row] : a.top_k_all;

@@ -428,6 +428,8 @@ def softmax_distill_grad(X_aug: torch.Tensor, W: torch.Tensor, b: torch.Tensor, 
     for v in (X_aug, idx, t):
         if not isinstance(v, torch.Tensor) or not v.is_cuda:
             raise ValueError("mlapi_amd.ops: inputs must be GPU tensors (no CPU fallback)")
+    if any(v is not None and v.device != X_aug.device for v in (W, b, idx, t, y)):
+        raise ValueError("softmax_distill_grad: all inputs must be on one device")
     if X_aug.dtype != torch.bfloat16 or W.dtype != torch.bfloat16 or b.dtype != torch.float32:
         raise TypeError("softmax_distill_grad: X_aug, W bf16 and b f32")
     if idx.dtype != torch.int32 or t.dtype not in _LOGIT_DT:
@@ -438,8 +440,8 @@ def softmax_distill_grad(X_aug: torch.Tensor, W: torch.Tensor, b: torch.Tensor, 
     if X_aug.stride(1) != 1 or ldx < F_aug or ldx % 8 != 0:
         raise ValueError("mlapi_amd.ops: X_aug rows must be contiguous with a row stride >= F_aug, a "
                          "multiple of 8")
-    if gemm_width(F) != F or F_aug != F + 8 or b.numel() != K:
-        raise ValueError("softmax_distill_grad: shape mismatch (W must be [K, Fk], X_aug [B, Fk + 8])")
+    if B < 1 or gemm_width(F) != F or F_aug != F + 8 or b.numel() != K:
+        raise ValueError("softmax_distill_grad: shape mismatch (W must be [K, Fk], X_aug [B, Fk + 8], B >= 1)")
     k = idx.shape[1] if idx.dim() == 2 else 0
     if idx.shape != (B, k) or t.shape != (B, k) or not 1 <= k <= MAX_TOP or (k > 1 and (idx.stride(1), t.stride(1)) != (1, 1)):
         raise ValueError(f"softmax_distill_grad: idx and t must be [B, k] with contiguous rows, 1 <= k <= {MAX_TOP}")

@@ -4,7 +4,8 @@ Each takes logits ``Z`` [B, K] (f32, bf16 or f16; B rows of one sample's K class
 :func:`mlapi_amd.ops.linear.gemm_logits` or any other model gives them, with contiguous columns and any row
 stride, and launches on the current stream of Z's device. They allocate their results and workspace from
 torch's allocator and do not synchronise, so they can be captured into a HIP graph. GPU tensors only;
-plain oracles are in :mod:`mlapi_amd.ops.reference`.
+plain oracles are in :mod:`mlapi_amd.ops.reference`. Gradients are results like any other: nothing here is recorded by
+autograd.
 
 The order of a row's classes is everywhere: larger logit first, then lower class. A class whose logit is
 -inf is masked; so is NaN in :func:`top_logits` and :func:`sample_logits`, while in the distillation loss a
@@ -84,6 +85,15 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + n * t.element_size()
 
 
+def _apart(name: str, outs, ins) -> None:
+    """Results given by the caller must not lie on inputs (which other rows' blocks may still read)."""
+    ins = [_span(v) for v in ins if isinstance(v, torch.Tensor)]
+    outs = [_span(v) for v in outs]
+    for i, (a, b) in enumerate(outs):
+        if any(a < q and p < b for p, q in ins + outs[:i]):
+            raise ValueError(f"{name}: out overlaps an input or another result")
+
+
 def _workspace(nbytes: int, device) -> Tuple[Optional[torch.Tensor], int]:
     """(the tensor that keeps it alive, its address)"""
     if nbytes == 0:
@@ -110,6 +120,7 @@ def top_logits(Z: torch.Tensor, k: int, out: Optional[Tuple[torch.Tensor, torch.
         for t, dt in ((values, Z.dtype), (idx, torch.int32)):
             if t.dtype != dt or t.shape != (B, k) or not t.is_contiguous() or t.device != Z.device:
                 raise ValueError("top_logits: out must be contiguous (Z's type [B, k], int32 [B, k]) on Z's device")
+        _apart("top_logits", out, (Z,))
     dt = _DT[Z.dtype]
     c = C()
     with _On(Z) as stream:
@@ -144,7 +155,10 @@ def _distill(name: str, Z, idx, t, temperature, alpha, y, *, g=None, stats_in=No
         raise ValueError(f"{name}: alpha below 1 mixes in hard labels and needs y")
     yp = 0 if y is None else _vector(name, "y", y, Z, torch.int32)
     gp = 0 if g is None else _vector(name, "g", g, Z, torch.float32)
-    pp = 0 if pred is None else _vector(name, "pred", pred, Z, torch.int32)
+    pp = 0
+    if pred is not None:
+        pp = _vector(name, "pred", pred, Z, torch.int32)
+        _apart(name, (pred,), (Z, idx, t, y, g))
     dt = ddt = _DT[Z.dtype]
     ldd = dp = 0
     if out is not None:
@@ -156,12 +170,7 @@ def _distill(name: str, Z, idx, t, temperature, alpha, y, *, g=None, stats_in=No
             raise ValueError(f"{name}: out must have contiguous, separate rows")
         ddt, dp = _DT[out.dtype], out.data_ptr()
         same = dp == Z.data_ptr() and ld == ldd and Z.dtype == out.dtype
-        for what, v in (("the logits without being the logits", Z), ("idx", idx), ("t", t), ("y", y), ("g", g),
-                        ("stats", stats_in), ("pred", pred)):
-            if v is not None and not (v is Z and same):
-                (a, b), (p, q) = _span(v), _span(out)
-                if a < q and p < b:
-                    raise ValueError(f"{name}: out overlaps {what}")
+        _apart(name, (out,), (None if same else Z, idx, t, y, g, stats_in, pred))
     elif dz:
         out = torch.empty((B, K), dtype=Z.dtype, device=dev)
         ldd, dp = K, out.data_ptr()
@@ -241,7 +250,8 @@ def sample_logits(Z: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.
     order (<= 0: all); of those, the classes whose preceding mass in the order is below ``top_p`` times their
     mass, the first always (>= 1: all); of those, the ones with w >= ``min_p`` (<= 0: all; the maximum has w = 1).
     The draw is the first class, counting up, whose cumulative kept mass exceeds u times the kept mass; ``prob`` is
-    its share of that mass. u is taken into [0, 1), a NaN as 0. A temperature of 0 takes the first maximum.
+    its share of that mass. u is taken into [0, 1), a NaN as 0. A temperature of 0 takes the first maximum; one of
+    infinity or NaN, in a tensor, counts as the largest finite number.
     A row whose classes are all masked gives (-1, 0).
 
     Each setting is one number for all rows, or a [B] tensor (f32; top_k int32) with one for each. Numbers are
@@ -249,7 +259,7 @@ def sample_logits(Z: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.
     always draw the same class."""
     B, K, ld = _logits("sample_logits", Z)
     up = _vector("sample_logits", "u", u, Z, torch.float32)
-    Tp, T = _setting("temperature", temperature, Z, torch.float32, float, float("inf"))
+    Tp, T = _setting("temperature", temperature, Z, torch.float32, float, torch.finfo(torch.float32).max)
     kp, k = _setting("top_k", top_k, Z, torch.int32, int, float("inf"))
     pp, p = _setting("top_p", top_p, Z, torch.float32, float, 1.0)
     mp, least = _setting("min_p", min_p, Z, torch.float32, float, 1.0)
@@ -261,6 +271,7 @@ def sample_logits(Z: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.
         idx, prob = out
         _vector("sample_logits", "out idx", idx, Z, torch.int32)
         _vector("sample_logits", "out prob", prob, Z, torch.float32)
+        _apart("sample_logits", out, (Z, u, temperature, top_k, top_p, min_p))
     dt = _DT[Z.dtype]
     c = C()
     with _On(Z) as stream:

@@ -150,6 +150,8 @@ def sample_ref(Z, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     col = lambda v: (v.float() if isinstance(v, torch.Tensor) else  # noqa: E731
                      torch.full((B,), float(v), dtype=torch.float32, device=Z.device)).double()[:, None]
     T, k, p, least = col(temperature), col(top_k), col(top_p), col(min_p).clamp(max=1.0)
+    most = torch.finfo(torch.float32).max
+    T = T.nan_to_num(most).clamp(max=most)
     m = z.amax(1, keepdim=True)
     live = z > -float("inf")
     x = torch.where(z == m, torch.zeros_like(z), (z - m) / T)

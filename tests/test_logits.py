@@ -168,5 +168,16 @@ def test_wrapper_refusals():
         ops.distill_grad(big[:60].view(3, 20), idx, t, stats, out=big[4:64].view(3, 20))
     with pytest.raises(ValueError):
         ops.distill_grad(Z, idx, t, stats, out=torch.zeros(3, 20, dtype=torch.float16, device=d))
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.sample_logits(Z, u, out=(torch.zeros(3, dtype=torch.int32, device=d), u))
+    k = torch.ones(3, dtype=torch.int32, device=d)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.sample_logits(Z, u, top_k=k, out=(k, torch.zeros(3, device=d)))
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.top_logits(Z, 2, out=(Z.view(-1)[:6].view(3, 2), torch.zeros(3, 2, dtype=torch.int32, device=d)))
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.distill_loss_grad(Z, idx, t, y=k, pred=k)
+    with pytest.raises(ValueError):
+        ops.sample_logits(Z, u, temperature=float("inf"))
     with pytest.raises(ValueError):
         ops.top_logits(Z, 2, out=(torch.zeros(3, 2, device=d), torch.zeros(3, 2, device=d)))

@@ -86,6 +86,24 @@ def test_distill(dtype, B, K, k, temperature, alpha):
         check_distill(Z, idx, t, temperature, alpha, y, g)
 
 
+@pytest.mark.parametrize("B,K", [(5, 1000), (3, 2048), (6, 1100), (2, 9000), (2, 150001)])
+def test_distill_longest_lists(B, K):
+    for k in (1000, 1024):
+        Z = rows(B, K, torch.float32, k, "bell", device=DEV)
+        idx, t = teacher(Z, k, 3, device=DEV)
+        y = torch.arange(B, dtype=torch.int32, device=DEV)
+        check_distill(Z, idx, t, 1.5, 0.6, y)
+
+
+def test_distill_one_list_for_all_rows():
+    """idx and t may be expanded: a row stride of 0."""
+    Z = rows(9, 700, torch.bfloat16, 2, "bell", device=DEV)
+    idx, t = teacher(Z[3:4], 6, 3, device=DEV)
+    loss, dz = ops.distill_loss_grad(Z, idx.expand(9, -1), t.expand(9, -1), temperature=2.0)
+    l2, d2 = ops.distill_loss_grad(Z, idx.repeat(9, 1), t.repeat(9, 1), temperature=2.0)
+    assert same(loss, l2) and same(dz, d2)
+
+
 def test_distill_nan_inf_and_classes_out_of_range():
     for K in (100, 3000, 70000):
         Z = rows(8, K, torch.float32, 1, "bell", device=DEV)
@@ -187,6 +205,27 @@ def test_sample_settings_per_row():
               top_p=torch.where(r % 4 == 0, 1.5, torch.rand(B, generator=g)),
               min_p=torch.where(r % 7 == 0, -1.0, 0.1 * torch.rand(B, generator=g)))
     check_sample(Z, torch.rand(B, generator=g).to(DEV), **{n: v.to(DEV) for n, v in kw.items()})
+
+
+@pytest.mark.parametrize("K", [50, 1900, 7000, 40000])
+def test_sample_infinite_temperatures_keep_masked_classes_out(K):
+    Z = rows(8, K, torch.float32, 12, "masked", device=DEV)
+    inf = torch.full((8,), INF, device=DEV)
+    inf[5] = float("nan")
+    u = torch.rand(8, generator=torch.Generator().manual_seed(1)).to(DEV)
+    for f in (dict(), dict(top_p=0.5), dict(top_k=20), dict(top_k=300, min_p=0.5)):
+        idx, _ = check_sample(Z, u, temperature=inf, **f)
+        assert idx[0] == -1 and (Z[torch.arange(1, 8), idx[1:].long()] > -INF).all()
+
+
+@pytest.mark.parametrize("K", [1500, 20000])
+def test_sample_list_lengths_of_all_kinds_in_one_batch(K):
+    B = 40
+    Z = rows(B, K, torch.bfloat16, 13, "bell", device=DEV)
+    k = torch.tensor([0, 1, 2, 63, 64, 65, 127, 128, 129, 255, 256, 257, 1023, K - 1, K, K + 5, -3] * 3)[:B].to(torch.int32)
+    u = torch.rand(B, generator=torch.Generator().manual_seed(2)).to(DEV)
+    check_sample(Z, u, top_k=k.to(DEV))
+    check_sample(Z, u, top_k=k.to(DEV), top_p=0.7, temperature=1.3)
 
 
 def test_sample_random_numbers_at_their_ends():
