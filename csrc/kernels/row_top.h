@@ -164,7 +164,8 @@ __device__ __forceinline__ int wave_top(const Held<T> (&raw)[NV], int lane, int 
 
 // ---- one block, row in memory -------------------------------------------------------------------
 constexpr int TOP_THREADS = 256;
-constexpr int BLOCK_TOP = 128;    // longest list
+constexpr int BLOCK_TOP = 256;    // longest list
+constexpr int THREAD_BOUND = 128; // longest list bounded by the threads' best places; longer ones: by the groups'
 constexpr int BLOCK_CAND = 1024;  // gathered classes
 constexpr int GROUP_LANES = 16;   // a group is 16 lanes' vectors of `rounds` steps: 256 bytes each
 constexpr int MAX_GROUPS = 2048;
@@ -244,9 +245,22 @@ __device__ __forceinline__ int block_top(const T* z, int c0, int c1, Places plac
   // one place: the bound need not be tight)
   const uint32_t key = order_key(best);
   const uint64_t mine = key > KEY_MASKED ? places.of(key, min(c0 + best_at * STEP + tid * V + V - 1, c1 - 1)) : 0;
-  const uint64_t bound = block_bound(mine, k, 32 + places.ib, s);
-  const float over = bound == 0 ? -__builtin_inff() : key_logit((uint32_t)(bound >> places.ib));
+  uint64_t bound = block_bound(mine, k, 32 + places.ib, s);
   const int ngroups = (steps + rounds - 1) / rounds * (TOP_THREADS / GROUP_LANES);
+  if (k > THREAD_BOUND) {
+    // 256 threads are too few groups for so many: the k-th largest of up to 2048 groups' logits, without their
+    // classes (ties of that logit are gathered too)
+    constexpr int PER = MAX_GROUPS / 64;
+    uint32_t v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int g = i * 64 + (tid & 63);
+      v[i] = g < ngroups ? order_key(s->u.g.most[g]) : 0;
+    }
+    const uint32_t key = kth_largest<PER, uint32_t>(v, k, 32);
+    bound = key > KEY_MASKED ? places.last(key) : 0;
+  }
+  const float over = bound == 0 ? -__builtin_inff() : key_logit((uint32_t)(bound >> places.ib));
   for (int i = tid; i < ngroups; i += TOP_THREADS)
     if (s->u.g.most[i] >= over) s->u.g.group[atomicAdd(&s->groups, 1)] = (uint16_t)i;
   __syncthreads();

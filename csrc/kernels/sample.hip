@@ -637,7 +637,7 @@ template <class T>
 Plan make_plan(const SampleCall& a) {
   Plan p;
   p.len = a.K;
-  if (a.top_k != nullptr || a.top_k_all < 1 || a.top_k_all > BLOCK_TOP) return p;
+  if (a.top_k != nullptr || a.top_k_all < 1 || a.top_k_all > THREAD_BOUND) return p;
   constexpr int STEP = TOP_THREADS * Vec<T>::N;
   const int steps = (a.K + STEP - 1) / STEP;
   const int64_t want = std::min<int64_t>({(512 + a.B - 1) / a.B, steps / 8, MERGE_PLACES / a.top_k_all, 64});

@@ -3,7 +3,7 @@
 // Bound by reading the logits once: one comparison per logit, and work on about k classes after it
 // (row_top.h). Short rows stay in one wave's registers, no barrier; a long row takes a block; a few long
 // rows are cut into parts whose sorted lists a second launch merges. Lists too long for those
-// (k > 256, long rows k > 128) are found by cutting the interval of places into bins (row_select.h).
+// (k > 256) are found by cutting the interval of places into bins (row_select.h).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -145,6 +145,8 @@ template <class T>
 Plan make_plan(int64_t B, int K, int k) {
   Plan p;
   constexpr int STEP = TOP_THREADS * Vec<T>::N;
+  p.len = K;
+  if (k > THREAD_BOUND) return p;  // the merge bounds lists by its threads
   const int steps = (K + STEP - 1) / STEP;
   const int64_t want = std::min<int64_t>({(512 + B - 1) / B, steps / 8, MERGE_PLACES / k, 64});
   p.parts = (int)std::max<int64_t>(1, want);
