@@ -55,26 +55,36 @@ struct Args {
 };
 
 // The listed classes of one row, in LDS: n = k entries, and the label as one more; 14 bytes each, so
-// that four rows of 1024 entries stay below 64 KB.
+// that four rows of 1024 entries (and 512 bytes of bits each) stay below 64 KB.
 struct Listed {
   int* cls;        // class, -1: absent
   float* lq;       // log2 q_j
   float* z;        // its logit; later the whole gradient of the class
   uint16_t* keep;  // whether this entry writes it
+  uint32_t* seen;  // a bit for every class (modulo their number): which have been listed
   __device__ Listed(unsigned char* lds, int cap) {
     cls = reinterpret_cast<int*>(lds);
     lq = reinterpret_cast<float*>(cls + cap);
     z = lq + cap;
     keep = reinterpret_cast<uint16_t*>(z + cap);
+    seen = reinterpret_cast<uint32_t*>(keep + cap);
   }
   static __host__ __device__ int capacity(int k) { return (k + 1 + 7) / 8 * 8; }
-  static __host__ __device__ size_t bytes(int k) { return (size_t)capacity(k) * 14; }
+  // 16 k^2 bits at most: two of k classes of a longer row share a bit by chance in 3 rows of 100, and
+  // the walk that then looks for the class twice costs time alone
+  static __host__ __device__ int bits(int k, int K) {
+    int n = 256;
+    while (n < K && n < 65536 && n < 16 * (k + 1) * (k + 1)) n *= 2;
+    return n;
+  }
+  static __host__ __device__ size_t bytes(int k, int K) { return (size_t)capacity(k) * 14 + bits(k, K) / 8; }
 };
 
 // Reads the row's entries (one wave): log2 q into lq (-inf: absent), logits into z. Returns Q (1, or 0 without entries; NaN
-// for a class out of range or a teacher's NaN or inf), and the label's weight (0 without one).
+// for a class out of range or a teacher's NaN or inf), the label's weight (0 without one), and whether
+// a class may stand twice.
 template <class T>
-__device__ void read_listed(const Args& a, int64_t row, int lane, Listed L, float& Q, float& H) {
+__device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane, Listed L, float& Q, float& H) {
   const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
   const int32_t* idx = a.idx + row * a.ldi;
   auto entry = [&](int j) -> float {
@@ -85,16 +95,40 @@ __device__ void read_listed(const Args& a, int64_t row, int lane, Listed L, floa
   };
   const float ct = 1.44269504088896340736f / a.T;
   float mt = -__builtin_inff();
-  int bad = 0;
-  for (int j = lane; j < a.k; j += 64) {
-    int c = idx[j];
-    const float x = entry(j);
-    if (c < 0 || x == -__builtin_inff()) c = -1;
-    if (c >= a.K) bad = 1, c = -1;
-    L.cls[j] = c;
-    L.lq[j] = x;
-    L.z[j] = c < 0 ? 0.f : (float)z[c];
-    if (c >= 0) mt = fmaxf(mt, x);
+  int bad = 0, twice = 0;
+  const int bits = Listed::bits(a.k, a.K);
+  for (int i = lane; i < bits / 32; i += 64) L.seen[i] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  auto see = [&](int c) {
+    const uint32_t b = 1u << (c & 31);
+    if (atomicOr(&L.seen[(c & (bits - 1)) >> 5], b) & b) twice = 1;
+  };
+  // four at a time: their loads wait for each other only at the gather
+  for (int j0 = lane; j0 < a.k; j0 += 256) {
+    int c[4];
+    float x[4], zc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + 64 * i;
+      c[i] = j < a.k ? idx[j] : -1;
+      x[i] = j < a.k ? entry(j) : -__builtin_inff();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (c[i] < 0 || x[i] == -__builtin_inff()) c[i] = -1;
+      if (c[i] >= a.K) bad = 1, c[i] = -1;
+      zc[i] = c[i] < 0 ? 0.f : (float)z[c[i]];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + 64 * i;
+      if (j < a.k) L.cls[j] = c[i], L.lq[j] = x[i], L.z[j] = zc[i];
+      if (c[i] >= 0) {
+        mt = fmaxf(mt, x[i]);
+        see(c[i]);
+      }
+    }
   }
   mt = finite_max(wave_max(mt));
   float s = 0.f;
@@ -117,9 +151,11 @@ __device__ void read_listed(const Args& a, int64_t row, int lane, Listed L, floa
   if (lane == 0) {
     L.cls[a.k] = c;
     L.z[a.k] = c < 0 ? 0.f : (float)z[c];
+    if (c >= 0) see(c);
     for (int j = a.k + 1; j < Listed::capacity(a.k); ++j) L.cls[j] = -1;
   }
   if (__any(bad)) Q = __builtin_nanf("");
+  return __any(twice);
 }
 
 // The row's loss (one wave; every lane gets it). Q and H as read_listed gave them.
@@ -153,9 +189,10 @@ __device__ __forceinline__ void dense_coeffs(const Args& a, float g, float Q, fl
 }
 
 // Whole gradients of the listed classes in [c0, c1), in the place of their logits; entries whose class
-// another entry writes, or that lie outside, are not kept. One wave.
-__device__ void listed_grads(const Args& a, int lane, Listed L, float g, float at, float a1, float m, float H,
-                             bool none, int c0, int c1) {
+// another entry writes, or that lie outside, are not kept. One wave. Only a list in which a class may
+// stand twice is walked for every entry.
+__device__ __forceinline__ void listed_grads(const Args& a, int lane, Listed L, bool twice, float g, float at, float a1,
+                                             float m, float H, bool none, int c0, int c1) {
   const float ct = 1.44269504088896340736f / a.T, c1e = 1.44269504088896340736f;
   const int cap = Listed::capacity(a.k);
   for (int j = lane; j <= a.k; j += 64) {
@@ -164,15 +201,19 @@ __device__ void listed_grads(const Args& a, int lane, Listed L, float g, float a
     float v = 0.f;
     if (mine) {
       float sum = 0.f;
-      for (int i = 0; i < cap; i += 4) {
-        const int4 o = *reinterpret_cast<const int4*>(L.cls + i);
-        const int oc[4] = {o.x, o.y, o.z, o.w};
+      if (!twice) {
+        sum = j == a.k ? H : a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[j]);
+      } else {
+        for (int i = 0; i < cap; i += 4) {
+          const int4 o = *reinterpret_cast<const int4*>(L.cls + i);
+          const int oc[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (oc[e] == c) {
-            if (i + e < j) mine = false;
-            sum += i + e == a.k ? H : a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[i + e]);
-          }
+          for (int e = 0; e < 4; ++e)
+            if (oc[e] == c) {
+              if (i + e < j) mine = false;
+              sum += i + e == a.k ? H : a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[i + e]);
+            }
+        }
       }
       const float d = L.z[j] - m;
       v = none ? at : at * __builtin_amdgcn_exp2f(d * ct) - g * sum;
@@ -196,13 +237,14 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
   const int64_t row = (int64_t)blockIdx.x * RPB + sub;
   if (row >= a.B) return;  // whole waves: rows of fewer than a block's threads have one wave, and no barrier
   const int K = a.K, cap = Listed::capacity(a.k);
-  Listed L(dyn + (size_t)sub * Listed::bytes(a.k), cap);
+  Listed L(dyn + (size_t)sub * Listed::bytes(a.k, a.K), cap);
   const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
   Held<T> raw[NV];
   load_row<T, NTR, NV>(raw, z, tid, K);
   float Q = 0.f, H = 0.f;
+  bool twice = false;
   if (tid < 64) {
-    read_listed<T>(a, row, lane, L, Q, H);
+    twice = read_listed<T>(a, row, lane, L, Q, H);
     if (NTR > 64 && lane == 0) bcast[sub][0] = Q, bcast[sub][1] = H;
   }
   auto sync = [] {
@@ -279,7 +321,7 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
       if (a.stats_out != nullptr) a.stats_out[row] = r;
       if (a.pred != nullptr) a.pred[row] = r.arg;
     }
-    if (a.dz != nullptr) listed_grads(a, lane, L, g, at, a1, m, H, r.st == 0.f, 0, K);
+    if (a.dz != nullptr) listed_grads(a, lane, L, twice, g, at, a1, m, H, r.st == 0.f, 0, K);
   }
   again();
   TO* dz = static_cast<TO*>(a.dz) + row * a.ldd;
@@ -468,7 +510,7 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
   float Q = 0.f, H = 0.f, at, a1;
   const int c0 = blockIdx.x * len, c1 = min(a.K, c0 + len);
   if (threadIdx.x < 64) {
-    read_listed<T>(a, row, lane, L, Q, H);
+    const bool twice = read_listed<T>(a, row, lane, L, Q, H);
     if (lane == 0) bcast[0] = Q, bcast[1] = H;
     dense_coeffs(a, g, Q, H, r, at, a1);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
@@ -483,7 +525,7 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
         if (a.pred != nullptr) a.pred[row] = r.arg;
       }
     }
-    if (a.dz != nullptr) listed_grads(a, lane, L, g, at, a1, m, H, r.st == 0.f, c0, c1);
+    if (a.dz != nullptr) listed_grads(a, lane, L, twice, g, at, a1, m, H, r.st == 0.f, c0, c1);
   }
   if (a.dz == nullptr) return;
   __syncthreads();
@@ -501,7 +543,7 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
 template <class T, class TO, int NTR, int NV>
 void launch_rows(const Args& a, hipStream_t stream) {
   constexpr int NT = NTR < 256 ? 256 : NTR, RPB = NT / NTR;
-  const size_t lds = RPB * Listed::bytes(a.k);
+  const size_t lds = RPB * Listed::bytes(a.k, a.K);
   hipLaunchKernelGGL((distill_rows_kernel<T, TO, NTR, NV>), dim3((unsigned)((a.B + RPB - 1) / RPB)), dim3(NT), lds,
                      stream, a);
   MLAPI_HIP_CHECK(hipGetLastError());
@@ -553,7 +595,7 @@ template <class T, class TO>
 void run_distill(Args a, RowStats* ws, hipStream_t stream) {
   const Plan p = make_plan<T>(a.B, a.K);
   if (p.parts == 0) return launch_resident<T, TO>(a, stream);
-  const size_t lds = Listed::bytes(a.k);
+  const size_t lds = Listed::bytes(a.k, a.K);
   a.parts = 1;
   for (int64_t r0 = 0; r0 < a.B; r0 += 65535) {  // grid.y holds 16 bits
     Args b = a;

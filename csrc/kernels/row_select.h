@@ -24,7 +24,7 @@ struct Places {
 struct Prefix {
   uint64_t cut;    // places >= cut are in it
   uint64_t count;  // classes in it
-  uint64_t mass;   // their weights
+  uint64_t mass;   // their weights (0 where the count was the target)
 };
 
 constexpr int SELECT_BINS = 1024;
@@ -41,7 +41,7 @@ struct SelectLds {
 // left: 1024 bins take one or two rounds for logits without many ties. A wave of its own (NT 64) needs no
 // barrier of its block.
 template <int NT, int BINS, class Each>
-__device__ __forceinline__ Prefix select_prefix(bool by_mass, uint64_t target, uint64_t lo, uint64_t hi,
+__device__ __forceinline__ Prefix select_prefix(const bool by_mass, uint64_t target, uint64_t lo, uint64_t hi,
                                                 SelectLds<BINS>* s, Each&& each) {
   constexpr int PER = BINS / 64, LOG = __builtin_ctz(BINS);
   const int tid = NT == 64 ? (int)threadIdx.x & 63 : (int)threadIdx.x;
@@ -65,7 +65,7 @@ __device__ __forceinline__ Prefix select_prefix(bool by_mass, uint64_t target, u
       if (place >= lo && place <= hi) {
         const int b = (int)((place - lo) >> sh);
         atomicAdd(&s->count[b], 1u);
-        atomicAdd((unsigned long long*)&s->mass[b], (unsigned long long)w);
+        if (by_mass) atomicAdd((unsigned long long*)&s->mass[b], (unsigned long long)w);
       }
     });
     sync();

@@ -535,7 +535,13 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Call a) {
     pass([&](float x, int) { valid += x > -__builtin_inff() ? 1 : 0; });
     valid = block_reduce<NT>(valid, reinterpret_cast<int*>(s.scratch), [](int x, int y) { return x + y; });
     if (set.top_k < valid) {
-      lo = select_prefix<NT, SELECT_BINS>(false, set.top_k, lo, hi, &s.u.select, each).cut;
+      auto places_only = [&](auto f) {
+        pass([&](float x, int i) {
+          const uint32_t key = order_key(x);
+          if (key > KEY_MASKED) f(places.of(key, i), (uint64_t)0);
+        });
+      };
+      lo = select_prefix<NT, SELECT_BINS>(false, set.top_k, lo, hi, &s.u.select, places_only).cut;
       keep.upto(lo, places);
       __syncthreads();
     }
