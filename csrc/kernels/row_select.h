@@ -21,6 +21,38 @@ struct Places {
   }
 };
 
+// the largest value that at least k of the wave's 64 M values reach (0 if none is): bit by bit, counted by
+// ballots, from `top` downwards. Stops early where exactly k values are left.
+template <int M, class U>
+__device__ __forceinline__ U kth_largest(const U (&v)[M], int k, int bits) {
+  U t = 0;
+  for (int b = bits - 1; b >= 0; --b) {
+    const U cand = t | ((U)1 << b);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < M; ++i) n += __popcll(__ballot(v[i] >= cand));
+    if (n >= k) t = cand;
+    if (n == k) break;
+  }
+  return t;
+}
+
+// A key that at least k classes of a row reach (0: fewer than k threads have a class): the k-th largest of
+// the largest keys of NT threads. `lds` holds NT values. What lies below needs no bin of select_prefix,
+// whose first round would else count most of a row in the few bins its exponents fall into.
+template <int NT>
+__device__ __forceinline__ uint32_t key_bound(uint32_t own, int k, uint32_t* lds) {
+  __syncthreads();
+  lds[threadIdx.x] = own > KEY_MASKED ? own : 0;
+  __syncthreads();
+  uint32_t v[NT / 64];
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) v[i] = lds[i * 64 + (threadIdx.x & 63)];
+  const uint32_t t = kth_largest<NT / 64, uint32_t>(v, k, 32);
+  __syncthreads();
+  return t;
+}
+
 struct Prefix {
   uint64_t cut;    // places >= cut are in it
   uint64_t count;  // classes in it

@@ -12,22 +12,6 @@
 namespace mlapi {
 namespace lrow {
 
-// the largest value that at least k of the wave's 64 M values reach (0 if none is): bit by bit, counted by
-// ballots, from `top` downwards. Stops early where exactly k values are left.
-template <int M, class U>
-__device__ __forceinline__ U kth_largest(const U (&v)[M], int k, int bits) {
-  U t = 0;
-  for (int b = bits - 1; b >= 0; --b) {
-    const U cand = t | ((U)1 << b);
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < M; ++i) n += __popcll(__ballot(v[i] >= cand));
-    if (n >= k) t = cand;
-    if (n == k) break;
-  }
-  return t;
-}
-
 // Ranks n distinct places in LDS (by how many are larger) over THREADS threads, each holding PER of them:
 // sorted[r] gets the place of rank r < k. Every place is read once by all, four at a time: `cand` is padded
 // with zeros to a multiple of four.

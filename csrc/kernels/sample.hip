@@ -512,6 +512,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Call a) {
   };
   float m = -__builtin_inff();
   pass([&](float x, int) { m = fmaxf(m, x); });
+  const float largest = m;  // this thread's
   m = block_reduce<NT>(m, reinterpret_cast<float*>(s.scratch), [](float x, float y) { return fmaxf(x, y); });
   if (m == -__builtin_inff() || !(set.T > 0.f)) {
     int first = K;
@@ -541,6 +542,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Call a) {
           if (key > KEY_MASKED) f(places.of(key, i), (uint64_t)0);
         });
       };
+      const uint32_t bound = key_bound<NT>(order_key(largest), set.top_k, s.u.select.count);
+      if (bound > KEY_MASKED) lo = places.last(bound);
       lo = select_prefix<NT, SELECT_BINS>(false, set.top_k, lo, hi, &s.u.select, places_only).cut;
       keep.upto(lo, places);
       __syncthreads();

@@ -100,6 +100,7 @@ __global__ __launch_bounds__(NT) void top_select_kernel(TopArgs a) {
       if (key > KEY_MASKED) hi = max(hi, key), lo = min(lo, key), ++n;
     }
   }
+  const uint32_t own = hi;  // this thread's largest
   hi = block_reduce<NT>(hi, scratch, [](uint32_t x, uint32_t y) { return max(x, y); });
   lo = block_reduce<NT>(lo, scratch, [](uint32_t x, uint32_t y) { return min(x, y); });
   n = block_reduce<NT>(n, scratch, [](uint32_t x, uint32_t y) { return x + y; });
@@ -118,6 +119,7 @@ __global__ __launch_bounds__(NT) void top_select_kernel(TopArgs a) {
       }
     }
   };
+  lo = max(lo, key_bound<NT>(own, take, sel.count));
   const Prefix p = select_prefix<NT, SELECT_BINS>(false, take, places.last(lo), places.first(hi) - 1, &sel, each);
   if (threadIdx.x == 0) found = 0;
   __syncthreads();
