@@ -332,3 +332,50 @@ def test_empty_batches():
     loss, dz = ops.distill_loss_grad(Z, idx, val)
     assert loss.shape == (0,) and dz.shape == (0, 50)
     assert ops.sample_logits(Z, torch.empty(0, device=DEV))[0].shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_most_classes(dtype):
+    K = 1 << 20
+    Z = rows(2, K, dtype, 3, "bell", device=DEV)
+    for k in (5, 200, 1000):
+        val, idx = ops.top_logits(Z, k)
+        rv, ri = ref.top_logits_ref(Z, k)
+        assert torch.equal(idx, ri) and same(val, rv)
+    for n, f in enumerate((dict(), dict(top_p=0.9), dict(top_k=40), dict(top_k=700, min_p=0.01), dict(temperature=2.0))):
+        check_sample(Z, torch.rand(2, generator=torch.Generator().manual_seed(n)).to(DEV), **f)
+    idx, t = teacher(Z, 100, 3, device=DEV)
+    check_distill(Z, idx, t, 2.0, 0.5, torch.tensor([K - 1, 0], dtype=torch.int32, device=DEV))
+
+
+def test_many_short_rows():
+    B = 70001
+    Z = rows(B, 3, torch.float16, 4, "ties", device=DEV)
+    val, idx = ops.top_logits(Z, 2)
+    rv, ri = ref.top_logits_ref(Z, 2)
+    assert torch.equal(idx, ri) and same(val, rv)
+    u = torch.rand(B, generator=torch.Generator().manual_seed(1)).to(DEV)
+    for f in (dict(), dict(top_p=0.6), dict(top_k=2)):
+        check_sample(Z, u, **f)
+    loss, dz = ops.distill_loss_grad(Z, idx, val, temperature=1.5)
+    rl, rd = ref.distill_ref(Z, idx, val, temperature=1.5)
+    # three terms of at most 8 each and their exponentials: 200 roundings of 2^-24; f16 gradients below 1.5 once more
+    assert ((loss.double() - rl).abs() <= 200 * 2.0 ** -24 * 8).all()
+    assert ((dz.double() - rd).abs() <= rd.abs() * 2.0 ** -11 + 200 * 2.0 ** -24 * 8 + 2.0 ** -25).all()
+
+
+def test_more_long_rows_than_a_grid_dimension():
+    """Rows that are cut into parts, past 65535 of them (17 GB, written in place)."""
+    B, K = 65539, 131077
+    src = rows(3, K, torch.bfloat16, 5, "bell", device=DEV)
+    idx, t = teacher(src, 8, 5, device=DEV)
+    loss, dz = ops.distill_loss_grad(src, idx, t, temperature=2.0)
+    Z = torch.zeros(B, K, dtype=torch.bfloat16, device=DEV)
+    Z[-3:] = src
+    idx, t = (torch.cat([v[:1].expand(B - 3, -1), v]) for v in (idx, t))
+    l2, d2 = ops.distill_loss_grad(Z, idx, t, temperature=2.0, out=Z)
+    assert (d2[:5].float().sum(1).abs() <= 2.0 ** -7 * 4).all()  # p - q, each entry rounded to bf16: half steps of 2 T
+    # the batch is cut into other parts than three rows are: the sums' trees differ
+    assert ((l2[-3:] - loss).abs() <= 1000 * 2.0 ** -24 * (loss.abs() + 8)).all()
+    d = (d2[-3:].double() - dz.double()).abs()
+    assert (d <= dz.double().abs() * 2.0 ** -7 + 1e-6).all()
