@@ -239,3 +239,17 @@ def test_distill_grad_refusals():
 
 def test_rows_helper_masks():
     assert (rows(2, 8, torch.float32, 0, "masked")[0] == -INF).all()
+
+
+def test_two_ranks_distil_as_one(tmp_path):
+    from test_distributed import run
+
+    script = str(ROOT / "tests" / "dist" / "distill_train.py")
+    for n in (1, 2):
+        run(n, script, {"OUT": str(tmp_path)})
+    one, a, b = (np.load(tmp_path / f"params_{n}.npy") for n in ("1_0", "2_0", "2_1"))
+    assert np.array_equal(a, b)
+    # the same gradient in two sums: f32 sums of 128 terms below 4, five steps whose momentum sums to at most 5 each
+    tol = 0.5 * 25 * 128 * 2.0 ** -24 * 4
+    assert np.abs(one - a).max() <= tol
+    assert abs(np.load(tmp_path / "loss_1_0.npy") - np.load(tmp_path / "loss_2_0.npy")) <= tol
