@@ -55,6 +55,7 @@ struct Args {
   int64_t B, ldz, ldi, ldt, ldd;
   int K, k, parts, t_dt;
   float T, soft, hard;  // soft = a, hard = 1 - a (0 without labels)
+  bool two;             // labels at a temperature other than the teacher's: a second softmax
 };
 
 // The listed classes of one row, in LDS: n = k entries, and the label as one more; 14 bytes each, so
@@ -292,7 +293,9 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
     r.st = block_reduce<NTR>(r.st, scratch, add2);
   }
   again();
-  if (!given && a.hard != 0.f) {
+  if (!given) r.s1 = a.hard != 0.f ? r.st : 0.f;
+  if (!given && a.two) {
+    r.s1 = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -331,6 +334,7 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
   if (a.dz != nullptr) {
     typedef TO out_t __attribute__((ext_vector_type(V), aligned(sizeof(TO))));
     const int whole = K / (NTR * V);
+    const float all = a.two ? at : at + a1;  // at T = 1 both softmaxes are one
     out_t last = {};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -339,8 +343,8 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float d = raw[v][e] - m;
-          float x = r.st == 0.f ? at : at * __builtin_amdgcn_exp2f(d * ct);
-          if (a.hard != 0.f) x += a1 * __builtin_amdgcn_exp2f(d * c1);
+          float x = r.st == 0.f ? at : all * __builtin_amdgcn_exp2f(d * ct);
+          if (a.two) x += a1 * __builtin_amdgcn_exp2f(d * c1);
           o[e] = (TO)x;
         }
         if (v < whole)
@@ -384,6 +388,7 @@ __device__ __forceinline__ RowStats stream_stats(const Args& a, const T* z, int 
   constexpr int V = Vec<T>::N, U = 4, STEP = NT * V;
   const float ct = 1.44269504088896340736f / a.T, ce = 1.44269504088896340736f;
   RowStats r{-__builtin_inff(), 0.f, 0.f, 0};
+#pragma unroll 1
   for (int base = c0; base < c1; base += U * STEP) {
     Held<T> raw[U];
 #pragma unroll
@@ -417,7 +422,7 @@ __device__ __forceinline__ RowStats stream_stats(const Args& a, const T* z, int 
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < V; ++e) r.st += __builtin_amdgcn_exp2f((raw[u][e] - mf) * ct);
-    if (a.hard != 0.f)
+    if (a.two)
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -434,6 +439,7 @@ __device__ __forceinline__ RowStats stream_stats(const Args& a, const T* z, int 
   r = part[0];
 #pragma unroll 1
   for (int w = 1; w < NT / 64; ++w) merge_stats(r, part[w], ct, ce);
+  if (!a.two) r.s1 = a.hard != 0.f ? r.st : 0.f;
   return r;
 }
 
@@ -455,6 +461,7 @@ __device__ __forceinline__ void stream_grad(const Args& a, const T* z, TO* dz, i
   typedef TO out_t __attribute__((ext_vector_type(V), aligned(sizeof(TO))));
   const float ct = 1.44269504088896340736f / a.T, ce = 1.44269504088896340736f, m = finite_max(r.m);
   const bool none = r.st == 0.f;
+  const float all = a.two ? at : at + a1;  // at T = 1 both softmaxes are one
   const int steps = (c1 - c0 + U * STEP - 1) / (U * STEP);
   for (int s = steps - 1; s >= 0; --s) {
     const int base = c0 + s * U * STEP;
@@ -474,8 +481,8 @@ __device__ __forceinline__ void stream_grad(const Args& a, const T* z, TO* dz, i
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float d = raw[u][e] - m;
-        float x = none ? at : at * __builtin_amdgcn_exp2f(d * ct);
-        if (a.hard != 0.f) x += a1 * __builtin_amdgcn_exp2f(d * ce);
+        float x = none ? at : all * __builtin_amdgcn_exp2f(d * ct);
+        if (a.two) x += a1 * __builtin_amdgcn_exp2f(d * ce);
         o[e] = (TO)x;
       }
       if (base + (u + 1) * STEP <= c1 || i + V <= c1) {
@@ -659,6 +666,7 @@ void launch_distill(const DistillCall& c, hipStream_t stream) {
   a.B = c.B, a.ldz = c.ldz, a.ldi = c.ldi, a.ldt = c.ldt, a.ldd = c.ldd;
   a.K = c.K, a.k = c.k, a.parts = 1, a.t_dt = c.t_dt;
   a.T = c.temperature, a.soft = c.alpha, a.hard = c.y != nullptr ? 1.f - c.alpha : 0.f;
+  a.two = a.hard != 0.f && c.temperature != 1.f;
   RowStats* ws = static_cast<RowStats*>(c.workspace);
   if (c.dt == DT_F32 && c.out_dt == DT_F32) return run_distill<float, float>(a, ws, stream);
   if (c.dt == DT_F32 && c.out_dt == DT_BF16) return run_distill<float, __bf16>(a, ws, stream);

@@ -73,7 +73,7 @@ def check_distill(Z, idx, t, temperature, alpha, y=None, g=None):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,K", SHAPES)
-@pytest.mark.parametrize("k,temperature,alpha", [(1, 1.0, 1.0), (8, 2.0, 1.0), (33, 0.7, 0.4), (65, 3.0, 0.0)])
+@pytest.mark.parametrize("k,temperature,alpha", [(1, 1.0, 1.0), (8, 2.0, 1.0), (33, 0.7, 0.4), (65, 3.0, 0.0), (12, 1.0, 0.5)])
 def test_distill(dtype, B, K, k, temperature, alpha):
     for n, kind in enumerate(["bell", "ties", "masked", "lowest", "flat"]):
         Z = rows(B, K, dtype, 3 * n + k, kind, pad=(0, 5)[n % 2], device=DEV)
