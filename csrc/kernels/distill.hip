@@ -86,7 +86,7 @@ struct Listed {
 
 // Reads the row's entries (one wave): log2 q into lq (-inf: absent), logits into z. Returns Q (1, or 0 without entries; NaN
 // for a class out of range or a teacher's NaN or inf), the label's weight (0 without one), and whether
-// a class may stand twice.
+// a class may stand twice among the entries.
 template <class T>
 __device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane, Listed L, float& Q, float& H) {
   const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
@@ -155,7 +155,6 @@ __device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane
   if (lane == 0) {
     L.cls[a.k] = c;
     L.z[a.k] = c < 0 ? 0.f : (float)z[c];
-    if (c >= 0) see(c);
     for (int j = a.k + 1; j < Listed::capacity(a.k); ++j) L.cls[j] = -1;
   }
   if (__any(bad)) Q = __builtin_nanf("");
@@ -194,34 +193,51 @@ __device__ __forceinline__ void dense_coeffs(const Args& a, float g, float Q, fl
 
 // Whole gradients of the listed classes in [c0, c1), in the place of their logits; entries whose class
 // another entry writes, or that lie outside, are not kept. One wave. Only a list in which a class may
-// stand twice is walked for every entry.
+// stand twice is walked for every entry (1501 x 32003 f16, k = 100: 27 us more).
 __device__ __forceinline__ void listed_grads(const Args& a, int lane, Listed L, bool twice, float g, float at, float a1,
                                              float m, float H, bool none, int c0, int c1) {
   const float ct = 1.44269504088896340736f / a.T, c1e = 1.44269504088896340736f;
-  const int cap = Listed::capacity(a.k);
+  const int cap = Listed::capacity(a.k), label = L.cls[a.k];
+  auto whole = [&](int j, float sum) {
+    const float d = L.z[j] - m;
+    float v = none ? at : at * __builtin_amdgcn_exp2f(d * ct) - g * sum;
+    if (!none && H != 0.f) v += a1 * __builtin_amdgcn_exp2f(d * c1e);
+    return v;
+  };
+  if (!twice) {  // the label, though, is often among the entries: one of them takes its weight along
+    bool listed = false;
+    for (int j = lane; j < a.k; j += 64) {
+      const int c = L.cls[j];
+      const bool mine = c >= c0 && c < c1, both = c >= 0 && c == label;
+      listed |= both;
+      L.keep[j] = mine ? 1 : 0;
+      if (mine) L.z[j] = whole(j, a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[j]) + (both ? H : 0.f));
+    }
+    listed = __any(listed);
+    if (lane == 0) {
+      const bool mine = label >= c0 && label < c1 && !listed;
+      L.keep[a.k] = mine ? 1 : 0;
+      if (mine) L.z[a.k] = whole(a.k, H);
+    }
+    return;
+  }
   for (int j = lane; j <= a.k; j += 64) {
     const int c = L.cls[j];
     bool mine = c >= c0 && c < c1;
     float v = 0.f;
     if (mine) {
       float sum = 0.f;
-      if (!twice) {
-        sum = j == a.k ? H : a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[j]);
-      } else {
-        for (int i = 0; i < cap; i += 4) {
-          const int4 o = *reinterpret_cast<const int4*>(L.cls + i);
-          const int oc[4] = {o.x, o.y, o.z, o.w};
+      for (int i = 0; i < cap; i += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(L.cls + i);
+        const int oc[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (oc[e] == c) {
-              if (i + e < j) mine = false;
-              sum += i + e == a.k ? H : a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[i + e]);
-            }
-        }
+        for (int e = 0; e < 4; ++e)
+          if (oc[e] == c) {
+            if (i + e < j) mine = false;
+            sum += i + e == a.k ? H : a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[i + e]);
+          }
       }
-      const float d = L.z[j] - m;
-      v = none ? at : at * __builtin_amdgcn_exp2f(d * ct) - g * sum;
-      if (!none && H != 0.f) v += a1 * __builtin_amdgcn_exp2f(d * c1e);
+      v = whole(j, sum);
     }
     L.z[j] = v;
     L.keep[j] = mine ? 1 : 0;
