@@ -18,9 +18,9 @@
 // Which kernel draws a row:
 //   rows of up to 2048 classes: one wave, from registers (sample_wave_kernel);
 //   longer rows with a short top-k: the k first classes by one pass (row_top.h), few long rows in parts;
-//   longer rows else: one block, from memory, two passes of weights (sample_row_kernel).
-// Bound by the issue of the weights' f64 instructions, 26 per logit: 65536 x 1000 f32 without filters 82 us (85 % of
-// it issue), p = 0.9: 175 us, k = 50: 149 us; 256 x 65537 bf16, p = 0.9: 73 us. By two launches where few rows
+//   longer rows else: one block, from memory, a pass of weights and one of those kept (sample_row_kernel).
+// Bound by the issue of the weights' f64 instructions, 26 per logit: 65536 x 1000 f32 without filters 79 us (85 % of
+// it issue), p = 0.9: 175 us, k = 50: 150 us; 256 x 65537 bf16, p = 0.9: 65 us. By two launches where few rows
 // have a short top-k: 1 x 131072 f32, k = 50: 16 us.
 #include <hip/hip_runtime.h>
 
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(TOP_THREADS) void sample_merge_kernel(Call a, int p
 // 256 rows of 65536 bf16 took 68 us with the row in registers, whose unrolled passes outgrow the
 // instruction cache.
 constexpr int MASS_LIST = 1024;
-template <int NT>
+template <class T, int NT>
 struct RowLds {
   // twice the threads: 65536 normal logits leave about 150 classes in the bin of a border
   static constexpr int BINS = NT < 512 ? 1024 : 2 * NT;
@@ -444,6 +444,7 @@ struct RowLds {
     uint64_t segment[SEGMENTS];
     SelectLds<SELECT_BINS> select;
   } u;
+  T kept[NT / 64][64 * Vec<T>::N];  // of a wave's vectors
   uint64_t scratch[NT / 64];
   uint64_t out[3];
   int n;
@@ -483,7 +484,7 @@ __device__ __forceinline__ void crossing(const uint64_t* x, int count, uint64_t*
 template <class T, int NT, bool SKIP>
 __global__ __launch_bounds__(NT) void sample_row_kernel(Call a) {
   constexpr int V = Vec<T>::N, STEP = NT * V, WAVES = NT / 64, U = 2;
-  typedef RowLds<NT> Lds;
+  typedef RowLds<T, NT> Lds;
   __shared__ Lds s;
   const int64_t row = blockIdx.x;
   const Settings set = settings(a, row);
@@ -574,19 +575,25 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Call a) {
     });
     const uint64_t above = s.out[1], target = s.out[2];
     const float near = (float)(int)s.out[0];
+    // the classes of that bin, still kept by top-k; their weights once they are few
+    const uint64_t from = lo;
     pass([&](float x, int i) {
       const float d = depth(x);
       if (d >= near && d < near + 1.f) {
-        const uint64_t w = first.mass(x, i);
-        if (w != 0) {
+        const uint32_t key = order_key(x);
+        const uint64_t place = places.of(key, i);
+        if (key > KEY_MASKED && place >= from) {
           const int j = atomicAdd(&s.n, 1);
-          if (j < MASS_LIST) s.u.h.place[j] = places.of(order_key(x), i), s.u.h.w[j] = w;
+          if (j < MASS_LIST) s.u.h.place[j] = place;
         }
       }
     });
     __syncthreads();
     const int n = s.n;
     if (n <= MASS_LIST) {
+      for (int j = tid; j < n; j += NT)
+        s.u.h.w[j] = weight(key_logit((uint32_t)(s.u.h.place[j] >> places.ib)), m, keep.c);
+      __syncthreads();
       for (int j = tid; j < n; j += NT) {
         const uint64_t mine = s.u.h.place[j], w = s.u.h.w[j];
         uint64_t before = above;
@@ -612,10 +619,39 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(Call a) {
       if (lane == 0) s.u.segment[i / (64 * V)] = w;
     });
   };
-  if (keep.all())
-    segments([&](float x, int) { return keep.any_mass(x); });
-  else
-    segments([&](float x, int i) { return keep.mass(x, i); });
+  if (keep.z == -__builtin_inff()) {
+    segments([&](float x, int) {
+      const uint64_t w = keep.any_mass(x);
+      return w >= keep.least ? w : 0;
+    });
+  } else {
+    // The classes kept of a vector, close together: a weight costs more than finding it a lane (256 x 65536
+    // bf16, p = 0.9, 1 class in 4 kept: 62 us, 70 with a weight for every class; with nearly all kept 78 and 75).
+    T* mine = s.kept[wave];
+    vectors([&](const Held<T>& h, int i) {
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float x = h[e];
+        const uint64_t in = __ballot(x > keep.z || (x == keep.z && i + e <= keep.cls));
+        const int at =
+            n + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+        if (in >> lane & 1) mine[at] = (T)x;
+        n += __popcll(in);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      uint64_t w = 0;
+      for (int j = 0; j < n; j += 64) {
+        const uint64_t wj = j + lane < n ? weight((float)mine[j + lane], m, keep.c) : 0;
+        w += wj >= keep.least ? wj : 0;
+      }
+      w = wave_sum_int(w);
+      if (lane == 0) s.u.segment[i / (64 * V)] = w;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    });
+  }
   __syncthreads();
   uint64_t total = 0;
   const int count = (K + STEP - 1) / STEP * WAVES;
