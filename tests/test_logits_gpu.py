@@ -228,6 +228,18 @@ def test_sample_list_lengths_of_all_kinds_in_one_batch(K):
     check_sample(Z, u, top_k=k.to(DEV), top_p=0.7, temperature=1.3)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [1900, 7001, 40000])
+def test_sample_border_among_weights_of_nothing(dtype, K):
+    """The last class kept has next to no weight, and thousands behind it have none at all."""
+    u = torch.tensor([0.0, 0.3, 0.7, 0.999, 1.0], device=DEV)
+    for kind in ("bell", "steep", "lowest", "odd", "ties"):
+        Z = rows(5, K, dtype, 14, kind, pad=1, device=DEV)
+        for f in (dict(), dict(top_k=900), dict(top_k=K - 1), dict(min_p=1e-3), dict(top_k=900, min_p=1e-12)):
+            for T in (0.02, 1.0, 1e4):
+                check_sample(Z, u, top_p=1 - 2.0 ** -24, temperature=T, **f)
+
+
 def test_sample_random_numbers_at_their_ends():
     """Four equal classes: u splits [0, 1) exactly in quarters; 1 and above, NaN and negative are taken in."""
     u = torch.tensor([0.0, 0.25, 0.5, 0.75, 1 - 2.0 ** -24, 1.0, 7.0, -1.0, float("nan"), 0.25 - 2.0 ** -26], device=DEV)
