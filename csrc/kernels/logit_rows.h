@@ -176,14 +176,14 @@ __device__ __forceinline__ U block_reduce(U v, U* scratch, Op op) {
 
 // ---- the order of a row's classes: larger logit first, then lower class -------------------------
 // An unsigned key that rises with the logit: -0 as +0; NaN as -inf. Masked classes (-inf, NaN) have
-// KEY_MASKED, every other key is larger.
-constexpr uint32_t KEY_MASKED = 0x007fffffu;
-__device__ __forceinline__ uint32_t order_key(float z) {
+// KEY_MASKED, every other key is larger. No logit has KEY_BELOW_ZERO, whose float is -0.
+constexpr uint32_t KEY_MASKED = 0x007fffffu, KEY_BELOW_ZERO = 0x7fffffffu;
+__host__ __device__ __forceinline__ uint32_t order_key(float z) {
   const uint32_t b = __builtin_bit_cast(uint32_t, z + 0.0f);
   const uint32_t key = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
   return z != z ? KEY_MASKED : key;
 }
-__device__ __forceinline__ float key_logit(uint32_t key) {
+__host__ __device__ __forceinline__ float key_logit(uint32_t key) {
   const uint32_t b = key ^ ((key & 0x80000000u) ? 0x80000000u : 0xffffffffu);
   return __builtin_bit_cast(float, b);
 }

@@ -10,14 +10,22 @@ namespace lrow {
 // Larger is earlier, no two classes share one.
 struct Places {
   int ib;  // bits of a class
-  __device__ explicit Places(int K) : ib(K <= 1 ? 1 : 32 - __builtin_clz((unsigned)(K - 1))) {}
-  __device__ __forceinline__ uint64_t of(uint32_t key, int i) const {
+  __host__ __device__ explicit Places(int K) : ib(K <= 1 ? 1 : 32 - __builtin_clz((unsigned)(K - 1))) {}
+  __host__ __device__ __forceinline__ uint64_t of(uint32_t key, int i) const {
     return ((uint64_t)key << ib) | (uint64_t)((1u << ib) - 1u - (unsigned)i);
   }
   __device__ __forceinline__ uint64_t first(uint32_t key) const { return ((uint64_t)key + 1) << ib; }  // exclusive
   __device__ __forceinline__ uint64_t last(uint32_t key) const { return (uint64_t)key << ib; }
-  __device__ __forceinline__ int cls(uint64_t place) const {
+  __host__ __device__ __forceinline__ int cls(uint64_t place) const {
     return (int)((1u << ib) - 1u - (unsigned)(place & ((1u << ib) - 1u)));
+  }
+  // The classes from a place upwards, told without their keys: those with x > z, or x == z and a class of at
+  // most `last`. A border that a search found may have a key that no logit has: past KEY_BELOW_ZERO, whose
+  // float equals the zeros above it, every zero is.
+  __host__ __device__ __forceinline__ void upto(uint64_t place, float& z, int& last) const {
+    const uint32_t key = (uint32_t)(place >> ib);
+    z = key_logit(key);
+    last = key == KEY_BELOW_ZERO ? 0x7fffffff : cls(place);
   }
 };
 

@@ -81,10 +81,7 @@ struct Keep {
     const uint64_t w = any_mass(x);
     return (x > z || (x == z && i <= cls)) && w >= least ? w : 0;
   }
-  __device__ __forceinline__ void upto(uint64_t place, Places places) {
-    z = key_logit((uint32_t)(place >> places.ib));
-    cls = places.cls(place);
-  }
+  __device__ __forceinline__ void upto(uint64_t place, Places places) { places.upto(place, z, cls); }
 };
 
 __device__ __forceinline__ Keep keep_all(float m, const Settings& set) {

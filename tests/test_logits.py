@@ -1,4 +1,8 @@
 """Oracles of the row operators over class logits, and the calls the operators refuse (no GPU needed)."""
+import shutil
+import subprocess
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -90,6 +94,20 @@ def test_sample_oracle_follows_the_definition():
 
 def test_rows_cover_what_they_name():
     assert rows(3, 50, torch.float32, 0, "odd").isnan().any() and (rows(3, 50, torch.float16, 0, "masked")[0] == -INF).all()
+
+
+@pytest.mark.skipif(not (Path("/opt/rocm/bin/hipcc").exists() or shutil.which("hipcc")), reason="needs hipcc")
+def test_a_border_between_places_keeps_whole_logits(tmp_path):
+    """csrc/tests/order_host.cpp: a filter's border may have a key that no logit has, the one below the zeros' among them."""
+    from mlapi_amd import _build
+
+    exe = tmp_path / "order_host"
+    src = _build.CSRC / "tests" / "order_host.cpp"
+    r = subprocess.run([_build.hipcc(), "-x", "hip", "--offload-host-only", "-O1", "-std=c++17", f"-I{_build.CSRC}", str(src),
+                        "-o", str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
 
 
 def test_cpu_tensors_are_refused(native):

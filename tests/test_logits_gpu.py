@@ -1,4 +1,6 @@
 """Row operators over class logits (top_logits, distill_*, sample_logits) against plain 64-bit forms."""
+import random
+
 import pytest
 import torch
 
@@ -238,6 +240,24 @@ def test_sample_border_among_weights_of_nothing(dtype, K):
         for f in (dict(), dict(top_k=900), dict(top_k=K - 1), dict(min_p=1e-3), dict(top_k=900, min_p=1e-12)):
             for T in (0.02, 1.0, 1e4):
                 check_sample(Z, u, top_p=1 - 2.0 ** -24, temperature=T, **f)
+
+
+@pytest.mark.parametrize("K,large,ones,k,p", [
+    (4096, 50, 1930, 2552, 0.945574164390564), (4096, 3, 1529, 3604, 0.8711135387420654),
+    (4096, 0, 1417, 2745, 0.9906483888626099), (8192, 0, 3005, 6398, 0.9207276105880737),
+    (4096, 0, 754, 3752, 0.956817090511322), (4096, 3, 1805, 2558, 0.9588007926940918)])
+def test_sample_borders_among_zeros_above_a_border_among_ties(K, large, ones, k, p):
+    """top-k ends among equal logits below zero and the nucleus among more zeros than its list holds, so that its
+    border is searched from one that lies between two logits: zeros of either sign are kept by their class alone."""
+    z = torch.zeros(K)
+    z[:large], z[K - ones:] = 2.0, -1.0
+    z[large:K - ones:2] = -0.0
+    z = z[torch.tensor(random.Random(K + large + ones).sample(range(K), K))]
+    u = torch.tensor([0.0, 0.2, 0.4, 0.6, 0.8, 0.999, 1.0], device=DEV)
+    for dtype in TYPES:
+        Z = z.to(dtype).to(DEV).expand(7, K).contiguous()
+        check_sample(Z, u, top_k=k, top_p=p)
+        check_sample(Z, u, top_k=torch.full((7,), k, dtype=torch.int32, device=DEV), top_p=p, min_p=0.3)
 
 
 def test_sample_random_numbers_at_their_ends():
