@@ -421,14 +421,16 @@ def softmax_distill_grad(X_aug: torch.Tensor, W: torch.Tensor, b: torch.Tensor, 
     teacher's top logits (``idx`` int32 [B, k], ``t`` [B, k]; :func:`mlapi_amd.ops.logits.top_logits`) as soft targets and
     the labels ``y`` at weight 1 - alpha (:func:`mlapi_amd.ops.logits.distill_loss` has the formula). Returns
     (dW_aug f32 [K, Fk + 8], stats f32 [loss_sum, n_correct]; n_correct is 0 without y). X_aug, W, b, ``update``
-    and ``p2p`` as there. ``ws``: a uint8 workspace of ``softmax_distill_workspace(B, K, Fk)`` bytes to keep."""
-    from mlapi_amd.ops.logits import _DT as _LOGIT_DT, MAX_TOP
+    and ``p2p`` as there. ``ws``: a uint8 workspace of ``softmax_distill_workspace(B, K, Fk)`` bytes to keep. Launches on
+    the current stream of X_aug's device, where all tensors must lie."""
+    from mlapi_amd.ops.logits import _DT as _LOGIT_DT, MAX_TOP, _On
 
     _check(W, b)
     for v in (X_aug, idx, t):
         if not isinstance(v, torch.Tensor) or not v.is_cuda:
             raise ValueError("mlapi_amd.ops: inputs must be GPU tensors (no CPU fallback)")
-    if any(v is not None and v.device != X_aug.device for v in (W, b, idx, t, y)):
+    dev = X_aug.device
+    if any(v is not None and v.device != dev for v in (W, b, idx, t, y)):
         raise ValueError("softmax_distill_grad: all inputs must be on one device")
     if X_aug.dtype != torch.bfloat16 or W.dtype != torch.bfloat16 or b.dtype != torch.float32:
         raise TypeError("softmax_distill_grad: X_aug, W bf16 and b f32")
@@ -449,30 +451,41 @@ def softmax_distill_grad(X_aug: torch.Tensor, W: torch.Tensor, b: torch.Tensor, 
         raise ValueError("softmax_distill_grad: y must be a contiguous int32 [B] GPU tensor")
     if alpha != 1.0 and y is None:
         raise ValueError("softmax_distill_grad: alpha below 1 mixes in hard labels and needs y")
+
+    def written(what, v, dtype, shape) -> int:
+        """The address of a tensor that the kernels write."""
+        if not isinstance(v, torch.Tensor) or v.device != dev or v.dtype != dtype or not v.is_contiguous() or \
+                (shape is not None and v.shape != shape):
+            raise ValueError(f"softmax_distill_grad: {what} must be a contiguous {dtype} "
+                             f"{'tensor' if shape is None else list(shape)} on {dev}")
+        return v.data_ptr()
+
     nbytes = C().softmax_distill_workspace(B, K, F)
     if ws is None:
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=X_aug.device)
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
     if stats_out is None:
-        stats_out = torch.zeros(2, dtype=torch.float32, device=X_aug.device)
+        stats_out = torch.zeros(2, dtype=torch.float32, device=dev)
     if dW_out is None:
-        dW_out = torch.empty(K, F_aug, dtype=torch.float32, device=X_aug.device)
-    if not dW_out.is_contiguous() or dW_out.shape != (K, F_aug) or dW_out.dtype != torch.float32:
-        raise ValueError("softmax_distill_grad: dW_out must be a contiguous f32 [K, Fk + 8] tensor")
+        dW_out = torch.empty(K, F_aug, dtype=torch.float32, device=dev)
+    wp = written("ws", ws, torch.uint8, None)
+    sp = written("stats_out", stats_out, torch.float32, (2,))
+    gp = written("dW_out", dW_out, torch.float32, (K, F_aug))
     upd = {}
     if update is not None:
-        p = update["params"]
-        if not p.is_contiguous() or p.shape != (K, F_aug) or p.dtype != torch.float32:
-            raise ValueError("softmax_distill_grad: update params must be a contiguous f32 [K, Fk + 8] tensor")
-        ptr = lambda v: 0 if v is None else v.data_ptr()  # noqa: E731
-        upd = dict(params=p.data_ptr(), mom=ptr(update.get("mom_buf")), shadow_w=ptr(update.get("shadow_w")),
-                   shadow_b=ptr(update.get("shadow_b")), pen_cols=F, lr=float(update["lr"]),
+        shapes = dict(mom_buf=(torch.float32, (K, F_aug)), shadow_w=(torch.bfloat16, (K, F)), shadow_b=(torch.float32, (K,)))
+        at = {n: 0 if update.get(n) is None else written(f"update {n}", update[n], *how) for n, how in shapes.items()}
+        upd = dict(params=written("update params", update["params"], torch.float32, (K, F_aug)), mom=at["mom_buf"],
+                   shadow_w=at["shadow_w"], shadow_b=at["shadow_b"], pen_cols=F, lr=float(update["lr"]),
                    inv_n=float(update["inv_n"]), l2=float(update.get("l2", 0.0)),
                    momentum=float(update.get("momentum", 0.0)))
-    C().softmax_distill(X_aug.data_ptr(), ldx, W.data_ptr(), b.data_ptr(), idx.data_ptr(),
-                        idx.stride(0) if B > 1 else k, t.data_ptr(), t.stride(0) if B > 1 else k, _LOGIT_DT[t.dtype], k,
-                        float(temperature), float(alpha), 0 if y is None else y.data_ptr(), B, F, K, dW_out.data_ptr(),
-                        stats_out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(), **upd,
-                        p2p=None if p2p is None else p2p.native, timeout_ms=int(timeout_ms))
+    if p2p is not None and p2p.device.index != dev.index:
+        raise ValueError(f"softmax_distill_grad: p2p is of {p2p.device}, the tensors are on {dev}")
+    with _On(X_aug) as stream:
+        C().softmax_distill(X_aug.data_ptr(), ldx, W.data_ptr(), b.data_ptr(), idx.data_ptr(),
+                            idx.stride(0) if B > 1 else k, t.data_ptr(), t.stride(0) if B > 1 else k, _LOGIT_DT[t.dtype], k,
+                            float(temperature), float(alpha), 0 if y is None else y.data_ptr(), B, F, K, gp, sp, wp,
+                            ws.numel(), stream, **upd, p2p=None if p2p is None else p2p.native,
+                            timeout_ms=int(timeout_ms))
     return dW_out, stats_out
 
 

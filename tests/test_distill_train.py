@@ -3,6 +3,7 @@ import json
 import subprocess
 import sys
 from pathlib import Path
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -235,6 +236,78 @@ def test_distill_grad_refusals():
             ops.softmax_distill_grad(*bad)
     with pytest.raises(TypeError):
         ops.softmax_distill_grad(Xa, W, b, idx.long(), t)
+
+
+class _Recorder:
+    """Stands in for the native module: takes the call and launches nothing."""
+
+    def __init__(self, native):
+        self.softmax_distill_workspace = native.softmax_distill_workspace
+        self.calls = []
+
+    def softmax_distill(self, *args, **kw):
+        self.calls.append((args, kw))
+
+
+@pytest.fixture
+def fake_gpus(native, monkeypatch):
+    """Two GPUs' tensors without storage, on a host without any: what is checked before a launch, and where it goes."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from mlapi_amd.ops import linear, logits
+
+    rec, log = _Recorder(native), []
+    monkeypatch.setattr(linear, "C", lambda: rec)
+    monkeypatch.setattr(linear, "_stream", lambda: log.append("current device's stream") or 7)
+    monkeypatch.setattr(logits, "_raw_stream", lambda index: 100 + index)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: log.append(d))
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        yield rec, log
+
+
+def _distill_call(dev, **kw):
+    from mlapi_amd.ops import linear as ops
+
+    e = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device=dev)  # noqa: E731
+    B, F, K, k = 4, 128, 5, 2
+    update = dict(params=e(K, F + 8), lr=0.1, inv_n=0.25, mom_buf=e(K, F + 8), shadow_w=e(K, F, dtype=torch.bfloat16),
+                  shadow_b=e(K))
+    update.update(kw.pop("update", {}))
+    args = dict(dW_out=e(K, F + 8), stats_out=e(2), ws=e(1 << 20, dtype=torch.uint8), update=update)
+    args.update(kw)
+    return ops.softmax_distill_grad(e(B, F + 8, dtype=torch.bfloat16), e(K, F, dtype=torch.bfloat16), e(K),
+                                    e(B, k, dtype=torch.int32), e(B, k), **args)
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+def test_distill_grad_launches_on_its_tensors_device(fake_gpus):
+    rec, log = fake_gpus
+    _distill_call("cuda:1")
+    assert len(rec.calls) == 1 and rec.calls[0][0][-1] == 101 and log == [1, 0]
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+@pytest.mark.parametrize("name,shape,dtype", [
+    ("ws", (1 << 20,), torch.uint8), ("dW_out", (5, 136), torch.float32), ("stats_out", (2,), torch.float32),
+    ("params", (5, 136), torch.float32), ("mom_buf", (5, 136), torch.float32), ("shadow_w", (5, 128), torch.bfloat16),
+    ("shadow_b", (5,), torch.float32)])
+def test_distill_grad_refuses_to_write_what_does_not_fit(fake_gpus, name, shape, dtype):
+    rec, _ = fake_gpus
+    bad = [torch.empty(shape, dtype=dtype, device="cpu"), torch.empty(shape, dtype=dtype, device="cuda:1"),
+           torch.empty(shape, dtype=torch.float64, device="cuda:0"),
+           torch.empty(*shape[:-1], 2 * shape[-1], dtype=dtype, device="cuda:0")[..., ::2]]
+    if name != "ws":  # its size is the launcher's to check
+        bad.append(torch.empty(*shape[:-1], shape[-1] - 1, dtype=dtype, device="cuda:0"))
+    for v in bad:
+        with pytest.raises(ValueError, match=name):
+            _distill_call("cuda:0", **({name: v} if name in ("ws", "dW_out", "stats_out") else dict(update={name: v})))
+    assert rec.calls == []
+
+
+def test_distill_grad_refuses_an_exchange_of_another_device(fake_gpus):
+    with pytest.raises(ValueError, match="p2p"):
+        _distill_call("cuda:0", p2p=SimpleNamespace(device=torch.device("cuda", 1), native=None))
 
 
 def test_rows_helper_masks():
