@@ -659,6 +659,7 @@ void run_distill(Args a, RowStats* ws, hipStream_t stream) {
 }  // namespace
 
 size_t distill_workspace(int dt, int64_t B, int K) {
+  if (B <= 0 || K < 1) return 0;
   const Plan p = dt == DT_F32 ? make_plan<float>(B, K) : make_plan<__bf16>(B, K);
   return (size_t)p.parts * (size_t)B * sizeof(RowStats);
 }

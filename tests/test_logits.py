@@ -149,6 +149,18 @@ def test_native_calls_refuse_before_any_launch(native):
         native.sample_logits(1, 0, 9, 4, 10, 0, 0, 1.0, 0, 0, 0, 1.0, 0, 0.0, 0, 0, 0, 0)
 
 
+@pytest.mark.parametrize("K", [1, 50, 40000, 200000, 1 << 20])
+def test_no_rows_need_no_workspace(native, K):
+    for dt in (1, 2, 3):
+        for B in (0, -1):
+            assert native.distill_workspace(dt, B, K) == 0
+            assert native.top_logits_workspace(dt, B, K, 8) == 0
+            assert native.sample_workspace(dt, B, K, False, 8) == 0
+    assert native.softmax_distill_workspace(0, K, 128) == 0
+    native.distill(dt=1, t_dt=1, out_dt=1, Z=0, ldz=K, B=0, K=K, idx=0, ldi=8, t=0, ldt=8, k=8, temperature=1.0, alpha=1.0,
+                   y=0, g=0, stats_in=0, loss=0, stats_out=0, pred=0, dz=0, ldd=K, ws=0, ws_bytes=0)
+
+
 @pytest.mark.gpu
 def test_wrapper_refusals():
     d = "cuda:0"

@@ -366,6 +366,18 @@ def test_empty_batches():
     assert ops.sample_logits(Z, torch.empty(0, device=DEV))[0].shape == (0,)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [40000, 200000])
+def test_empty_batches_of_long_rows(dtype, K):
+    Z = torch.empty(0, K, dtype=dtype, device=DEV)
+    val, idx = ops.top_logits(Z, 4)
+    loss, stats = ops.distill_loss(Z, idx, val)
+    dz = ops.distill_grad(Z, idx, val, stats)
+    l2, d2 = ops.distill_loss_grad(Z, idx, val, temperature=2.0)
+    assert loss.shape == l2.shape == (0,) and dz.shape == d2.shape == (0, K)
+    assert ops.sample_logits(Z, torch.empty(0, device=DEV), top_k=5)[0].shape == (0,)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_most_classes(dtype):
     K = 1 << 20
