@@ -137,7 +137,9 @@ __device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane
   mt = finite_max(wave_max(mt));
   float s = 0.f;
   for (int j = lane; j < a.k; j += 64) {
-    const float x = L.cls[j] < 0 ? -__builtin_inff() : (L.lq[j] - mt) * ct;
+    // a logit near the type's lowest has no q but a finite logarithm of it: -inf times 0 is no number
+    float x = (L.lq[j] - mt) * ct;
+    x = L.cls[j] < 0 ? -__builtin_inff() : x < -1e30f ? -1e30f : x;
     L.lq[j] = x;
     s += __builtin_amdgcn_exp2f(x);
   }
@@ -168,15 +170,16 @@ __device__ float row_loss(const Args& a, int lane, Listed L, float Q, float H, R
   float soft = 0.f;
   if (a.soft != 0.f) {
     // T times every term, so that no finite logit overflows in a quotient by T; q as 2^64 q, so that
-    // a q below the type's range still counts against a logit near the type's lowest value
-    const float lst = a.T * __logf(r.st), ln2_T = a.T * 0.693147180559945309f;
+    // a q below the type's range still counts against a logit near the type's lowest value; the factor of a
+    // term, not of their sum, which may pass the largest number where the loss does not
+    const float lst = a.T * __logf(r.st), ln2_T = a.T * 0.693147180559945309f, scale = a.soft * a.T;
     for (int j = lane; j < a.k; j += 64) {
       if (L.cls[j] < 0) continue;
       const float term = L.lq[j] * ln2_T - ((L.z[j] - m) - lst);
       soft += L.z[j] == -__builtin_inff() ? __builtin_inff()
-                                          : (term * 0x1p-64f) * __builtin_amdgcn_exp2f(L.lq[j] + 64.f);
+                                          : (term * 0x1p-64f) * (__builtin_amdgcn_exp2f(L.lq[j] + 64.f) * scale);
     }
-    soft = wave_sum(soft) * (a.soft * a.T);
+    soft = wave_sum(soft);
   }
   float loss = soft;
   if (H != 0.f) loss += H * (__logf(r.s1) - (L.z[a.k] - m));

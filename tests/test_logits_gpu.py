@@ -4,7 +4,7 @@ import random
 import pytest
 import torch
 
-from logits_cases import INF, distill_bounds, rows, teacher
+from logits_cases import INF, LOWEST, distill_bounds, rows, teacher
 from mlapi_amd.ops import logits as ops
 from mlapi_amd.ops import reference as ref
 
@@ -86,6 +86,34 @@ def test_distill(dtype, B, K, k, temperature, alpha):
             y = torch.randint(-1, K, (B,), generator=gen).to(torch.int32).to(DEV)
             g = (torch.rand(B, generator=gen) * 2 - 1).to(DEV)
         check_distill(Z, idx, t, temperature, alpha, y, g)
+
+
+@pytest.mark.parametrize("temperature", [0.01, 0.7, 1.0, 1.4, 2.0])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [9, 3000, 70001])
+def test_distill_lists_with_logits_of_the_types_lowest(K, dtype, temperature):
+    """A teacher that masks with its type's lowest logit lists such classes wherever fewer than k are left."""
+    k = min(K, 40)
+    Zt = torch.full((5, K), LOWEST[dtype])
+    Zt[1:, ::max(2, K // 7)] = rows(4, len(range(0, K, max(2, K // 7))), torch.float32, 3)
+    Zt = Zt.to(dtype).to(DEV)
+    t, idx = ops.top_logits(Zt, k)
+    assert (t.double().min(1).values == LOWEST[dtype]).all()
+    y = torch.tensor([0, 3, -1, K - 1, 2], dtype=torch.int32, device=DEV)
+    g = torch.full((5,), -0.5, device=DEV)
+    Z = rows(5, K, dtype, 4, "bell", device=DEV)
+    loss, dz = check_distill(Z, idx, t, temperature, 1.0)
+    assert loss.isfinite().all() and dz.isfinite().all()
+    check_distill(Z, idx, t, temperature, 0.3, y, g)
+    # a student that masks so too: its loss may be past the largest f32, whose place +inf takes
+    Z = rows(5, K, dtype, 4, "lowest", device=DEV)
+    kw = dict(temperature=temperature, alpha=0.3, y=y)
+    rl, rd = (v.cpu() for v in ref.distill_ref(Z, idx, t, g=g, **kw))
+    tl, td = distill_bounds(Z.cpu(), idx.cpu(), t.cpu(), rl, rd, temperature=temperature, alpha=0.3, y=y.cpu(), g=g.cpu())
+    loss, dz = (v.double().cpu() for v in ops.distill_loss_grad(Z, idx, t, g=g, **kw))
+    past = rl + tl > torch.finfo(torch.float32).max
+    assert ((loss - rl).abs() <= tl)[~past].all() and ((loss == INF) | (loss >= rl - tl))[past].all(), (loss, rl, tl)
+    assert ((dz - rd).abs() <= td).all()
 
 
 @pytest.mark.parametrize("B,K", [(5, 1000), (3, 2048), (6, 1100), (2, 9000), (2, 150001)])
