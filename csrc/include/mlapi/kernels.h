@@ -380,7 +380,8 @@ void launch_top_logits(int dt, const void* Z, int64_t ldz, int64_t B, int K, int
 // Distillation from a teacher's top logits (formulas: distill.hip). idx int32 [B, k] and t [B, k]
 // with row strides; y int32 [B] or null; g f32 [B] or null (1). Any of loss f32 [B], stats_out
 // (16 bytes per row), pred int32 [B] (first maximum), dz [B, K] may be null. With stats_in (an
-// earlier call's stats_out on the same Z, temperature and alpha) the row sums are not computed again.
+// earlier call's stats_out on the same Z, temperature and alpha) the row sums are not computed again, but
+// above a temperature of 16, where they take 64 bits.
 struct DistillCall {
   int dt = 0, t_dt = 0, out_dt = 0;
   const void* Z = nullptr;

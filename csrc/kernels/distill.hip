@@ -62,14 +62,14 @@ struct Args {
 // that four rows of 1024 entries (and 512 bytes of bits each) stay below 64 KB.
 struct Listed {
   int* cls;        // class, -1: absent
-  float* lq;       // log2 q_j
+  float* x;        // (t_j - max t) log2(e) / T; q_j = 2^x_j / S
   float* z;        // its logit; later the whole gradient of the class
   uint16_t* keep;  // whether this entry writes it
   uint32_t* seen;  // a bit for every class (modulo their number): which have been listed
   __device__ Listed(unsigned char* lds, int cap) {
     cls = reinterpret_cast<int*>(lds);
-    lq = reinterpret_cast<float*>(cls + cap);
-    z = lq + cap;
+    x = reinterpret_cast<float*>(cls + cap);
+    z = x + cap;
     keep = reinterpret_cast<uint16_t*>(z + cap);
     seen = reinterpret_cast<uint32_t*>(keep + cap);
   }
@@ -84,19 +84,21 @@ struct Listed {
   static __host__ __device__ size_t bytes(int k, int K) { return (size_t)capacity(k) * 14 + bits(k, K) / 8; }
 };
 
-// Reads the row's entries (one wave): log2 q into lq (-inf: absent), logits into z. Returns Q (1, or 0 without entries; NaN
-// for a class out of range or a teacher's NaN or inf), the label's weight (0 without one), and whether
-// a class may stand twice among the entries.
+// Logit j of the teacher's list of a row.
+__device__ __forceinline__ float teacher_logit(const Args& a, int64_t row, int j) {
+  const int64_t at = row * a.ldt + j;
+  if (a.t_dt == DT_F32) return static_cast<const float*>(a.t)[at];
+  if (a.t_dt == DT_BF16) return (float)static_cast<const __bf16*>(a.t)[at];
+  return (float)static_cast<const _Float16*>(a.t)[at];
+}
+
+// Reads the row's entries (one wave): x (-inf: absent) and logits into z. Returns S (0 without entries), Q (1, or 0
+// without entries; NaN for a class out of range or a teacher's NaN or inf), the label's weight (0 without one), and
+// whether a class may stand twice among the entries.
 template <class T>
-__device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane, Listed L, float& Q, float& H) {
+__device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane, Listed L, float& S, float& Q, float& H) {
   const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
   const int32_t* idx = a.idx + row * a.ldi;
-  auto entry = [&](int j) -> float {
-    const int64_t at = row * a.ldt + j;
-    if (a.t_dt == DT_F32) return static_cast<const float*>(a.t)[at];
-    if (a.t_dt == DT_BF16) return (float)static_cast<const __bf16*>(a.t)[at];
-    return (float)static_cast<const _Float16*>(a.t)[at];
-  };
   const float ct = 1.44269504088896340736f / a.T;
   float mt = -__builtin_inff();
   int bad = 0, twice = 0;
@@ -116,7 +118,7 @@ __device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane
     for (int i = 0; i < 4; ++i) {
       const int j = j0 + 64 * i;
       c[i] = j < a.k ? idx[j] : -1;
-      x[i] = j < a.k ? entry(j) : -__builtin_inff();
+      x[i] = j < a.k ? teacher_logit(a, row, j) : -__builtin_inff();
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -127,7 +129,7 @@ __device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int j = j0 + 64 * i;
-      if (j < a.k) L.cls[j] = c[i], L.lq[j] = x[i], L.z[j] = zc[i];
+      if (j < a.k) L.cls[j] = c[i], L.x[j] = x[i], L.z[j] = zc[i];
       if (c[i] >= 0) {
         mt = fmaxf(mt, x[i]);
         see(c[i]);
@@ -135,18 +137,16 @@ __device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane
     }
   }
   mt = finite_max(wave_max(mt));
-  float s = 0.f;
+  S = 0.f;
   for (int j = lane; j < a.k; j += 64) {
     // a logit near the type's lowest has no q but a finite logarithm of it: -inf times 0 is no number
-    float x = (L.lq[j] - mt) * ct;
+    float x = (L.x[j] - mt) * ct;
     x = L.cls[j] < 0 ? -__builtin_inff() : x < -1e30f ? -1e30f : x;
-    L.lq[j] = x;
-    s += __builtin_amdgcn_exp2f(x);
+    L.x[j] = x;
+    S += __builtin_amdgcn_exp2f(x);
   }
-  s = wave_sum(s);
-  const float ls = s == 0.f ? 0.f : __builtin_amdgcn_logf(s);
-  for (int j = lane; j < a.k; j += 64) L.lq[j] -= ls;
-  Q = s == 0.f ? 0.f : s / s;
+  S = wave_sum(S);
+  Q = S == 0.f ? 0.f : S / S;
   H = 0.f;
   int c = -1;
   if (a.hard != 0.f) {
@@ -163,21 +163,23 @@ __device__ __forceinline__ bool read_listed(const Args& a, int64_t row, int lane
   return __any(twice);
 }
 
-// The row's loss (one wave; every lane gets it). Q and H as read_listed gave them.
-__device__ float row_loss(const Args& a, int lane, Listed L, float Q, float H, RowStats r) {
+// The row's loss (one wave; every lane gets it). S, Q and H as read_listed gave them.
+__device__ float row_loss(const Args& a, int lane, Listed L, float S, float Q, float H, RowStats r) {
   if (r.st == 0.f) return Q != Q ? Q : 0.f;  // no class at all
   const float m = finite_max(r.m);
   float soft = 0.f;
-  if (a.soft != 0.f) {
-    // T times every term, so that no finite logit overflows in a quotient by T; q as 2^64 q, so that
-    // a q below the type's range still counts against a logit near the type's lowest value; the factor of a
-    // term, not of their sum, which may pass the largest number where the loss does not
-    const float lst = a.T * __logf(r.st), ln2_T = a.T * 0.693147180559945309f, scale = a.soft * a.T;
+  if (a.soft != 0.f && S != 0.f) {
+    // T times every term, so that no finite logit overflows in a quotient by T; the sums' logarithm of their ratio: both
+    // are near ln K at a high T, and what either is off counts T^2 times; a q below the type's range as 2^64 q, so
+    // that it still counts against a logit near the type's lowest value; the factor of a term, not of their sum,
+    // which may pass the largest number where the loss does not
+    const float ratio = a.T * __logf(r.st / S), ln2_T = a.T * 0.693147180559945309f, scale = a.soft * a.T / S;
     for (int j = lane; j < a.k; j += 64) {
       if (L.cls[j] < 0) continue;
-      const float term = L.lq[j] * ln2_T - ((L.z[j] - m) - lst);
-      soft += L.z[j] == -__builtin_inff() ? __builtin_inff()
-                                          : (term * 0x1p-64f) * (__builtin_amdgcn_exp2f(L.lq[j] + 64.f) * scale);
+      const float term = L.x[j] * ln2_T - ((L.z[j] - m) - ratio);
+      const bool low = L.x[j] < -64.f;
+      const float q = __builtin_amdgcn_exp2f(low ? L.x[j] + 64.f : L.x[j]) * scale;
+      soft += L.z[j] == -__builtin_inff() ? __builtin_inff() : (low ? term * 0x1p-64f : term) * q;
     }
     soft = wave_sum(soft);
   }
@@ -198,8 +200,9 @@ __device__ __forceinline__ void dense_coeffs(const Args& a, float g, float Q, fl
 // another entry writes, or that lie outside, are not kept. One wave. Only a list in which a class may
 // stand twice is walked for every entry (1501 x 32003 f16, k = 100: 27 us more).
 __device__ __forceinline__ void listed_grads(const Args& a, int lane, Listed L, bool twice, float g, float at, float a1,
-                                             float m, float H, bool none, int c0, int c1) {
+                                             float m, float S, float H, bool none, int c0, int c1) {
   const float ct = 1.44269504088896340736f / a.T, c1e = 1.44269504088896340736f;
+  const float scale = S == 0.f ? 0.f : a.soft * a.T / S;
   const int cap = Listed::capacity(a.k), label = L.cls[a.k];
   auto whole = [&](int j, float sum) {
     const float d = L.z[j] - m;
@@ -214,7 +217,7 @@ __device__ __forceinline__ void listed_grads(const Args& a, int lane, Listed L, 
       const bool mine = c >= c0 && c < c1, both = c >= 0 && c == label;
       listed |= both;
       L.keep[j] = mine ? 1 : 0;
-      if (mine) L.z[j] = whole(j, a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[j]) + (both ? H : 0.f));
+      if (mine) L.z[j] = whole(j, scale * __builtin_amdgcn_exp2f(L.x[j]) + (both ? H : 0.f));
     }
     listed = __any(listed);
     if (lane == 0) {
@@ -237,7 +240,7 @@ __device__ __forceinline__ void listed_grads(const Args& a, int lane, Listed L, 
         for (int e = 0; e < 4; ++e)
           if (oc[e] == c) {
             if (i + e < j) mine = false;
-            sum += i + e == a.k ? H : a.soft * a.T * __builtin_amdgcn_exp2f(L.lq[i + e]);
+            sum += i + e == a.k ? H : scale * __builtin_amdgcn_exp2f(L.x[i + e]);
           }
       }
       v = whole(j, sum);
@@ -264,10 +267,10 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
   const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
   Held<T> raw[NV];
   load_row<T, NTR, NV>(raw, z, tid, K);
-  float Q = 0.f, H = 0.f;
+  float S = 0.f, Q = 0.f, H = 0.f;
   bool twice = false;
   if (tid < 64) {
-    twice = read_listed<T>(a, row, lane, L, Q, H);
+    twice = read_listed<T>(a, row, lane, L, S, Q, H);
     if (NTR > 64 && lane == 0) bcast[sub][0] = Q, bcast[sub][1] = H;
   }
   auto sync = [] {
@@ -339,14 +342,14 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
   dense_coeffs(a, g, Q, H, r, at, a1);
   if (tid < 64) {
     if (a.loss != nullptr) {
-      const float loss = row_loss(a, lane, L, Q, H, r);
+      const float loss = row_loss(a, lane, L, S, Q, H, r);
       if (lane == 0) a.loss[row] = loss;
     }
     if (lane == 0) {
       if (a.stats_out != nullptr) a.stats_out[row] = r;
       if (a.pred != nullptr) a.pred[row] = r.arg;
     }
-    if (a.dz != nullptr) listed_grads(a, lane, L, twice, g, at, a1, m, H, r.st == 0.f, 0, K);
+    if (a.dz != nullptr) listed_grads(a, lane, L, twice, g, at, a1, m, S, H, r.st == 0.f, 0, K);
   }
   again();
   TO* dz = static_cast<TO*>(a.dz) + row * a.ldd;
@@ -536,17 +539,17 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
     r = RowStats{__shfl(r.m, 0, 64), __shfl(r.st, 0, 64), __shfl(r.s1, 0, 64), __shfl(r.arg, 0, 64)};
   }
   const float m = finite_max(r.m), g = a.g != nullptr ? a.g[row] : 1.f;
-  float Q = 0.f, H = 0.f, at, a1;
+  float S = 0.f, Q = 0.f, H = 0.f, at, a1;
   const int c0 = blockIdx.x * len, c1 = min(a.K, c0 + len);
   if (threadIdx.x < 64) {
-    const bool twice = read_listed<T>(a, row, lane, L, Q, H);
+    const bool twice = read_listed<T>(a, row, lane, L, S, Q, H);
     if (lane == 0) bcast[0] = Q, bcast[1] = H;
     dense_coeffs(a, g, Q, H, r, at, a1);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
     if (blockIdx.x == 0) {
       if (a.loss != nullptr) {
-        const float loss = row_loss(a, lane, L, Q, H, r);
+        const float loss = row_loss(a, lane, L, S, Q, H, r);
         if (lane == 0) a.loss[row] = loss;
       }
       if (lane == 0) {
@@ -554,7 +557,7 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
         if (a.pred != nullptr) a.pred[row] = r.arg;
       }
     }
-    if (a.dz != nullptr) listed_grads(a, lane, L, twice, g, at, a1, m, H, r.st == 0.f, c0, c1);
+    if (a.dz != nullptr) listed_grads(a, lane, L, twice, g, at, a1, m, S, H, r.st == 0.f, c0, c1);
   }
   if (a.dz == nullptr) return;
   __syncthreads();
@@ -568,7 +571,226 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
     if (L.keep[j] != 0) dz[L.cls[j]] = (TO)L.z[j];
 }
 
+// ---- high temperatures --------------------------------------------------------------------------
+// A list of every class leaves p and q only (z - t) / T apart, while the loss, T^2 times a difference of their
+// logarithms, stays of the size of (z - t)^2: what an f32 sum is off, about 2^-22, counts T^2 times (6e-5 at T = 16),
+// and T times in the gradient of a listed class. Above, the sums, the listed classes and the loss are evaluated in
+// 64 bits, T^2 2^-50; the dense part, where nothing cancels, is not. One block to a row, which it reads three times, the
+// last two from the caches where it is not too long; bound by 64-bit exponentials, one a logit (two with labels).
+// 65536 x 1000 f32 with labels: 257 us, 108 at T <= 16; 2048 x 65536 bf16: 353 and 114; 7 x 200001 f32: 87 and 16.
+constexpr float HOT_T = 16.f;
+
+// The listed classes of one row, in LDS: n = k entries, and the label as one more.
+struct HotListed {
+  double* q;       // exp((t_j - max t) / T), 0: absent
+  int* cls;        // class, -1: absent
+  float *t, *z;    // its logits; z later the whole gradient of the class
+  uint16_t* keep;  // whether this entry writes it
+  uint32_t* seen;  // as Listed's
+  __device__ HotListed(unsigned char* lds, int cap) {
+    q = reinterpret_cast<double*>(lds);
+    cls = reinterpret_cast<int*>(q + cap);
+    t = reinterpret_cast<float*>(cls + cap);
+    z = t + cap;
+    keep = reinterpret_cast<uint16_t*>(z + cap);
+    seen = reinterpret_cast<uint32_t*>(keep + cap);
+  }
+  static __host__ __device__ size_t bytes(int k, int K) {
+    return (size_t)Listed::capacity(k) * 22 + Listed::bits(k, K) / 8;
+  }
+};
+
+template <class T, class TO, int NT>
+__global__ __launch_bounds__(NT) void distill_hot_kernel(Args a) {
+  constexpr int V = Vec<T>::N, STEP = NT * V;
+  __shared__ double scratch[NT / 64];
+  extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
+  const int64_t row = blockIdx.x;
+  const int K = a.K, k = a.k, tid = threadIdx.x, cap = Listed::capacity(k);
+  const double rT = 1.0 / (double)a.T;
+  const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
+  const int32_t* idx = a.idx + row * a.ldi;
+  HotListed L(dyn, cap);
+  auto sync = [] {
+    if constexpr (NT > 64) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  auto fmax2 = [](float x, float y) { return fmaxf(x, y); };
+  auto sum = [&](double v) {  // over the block, to all its threads
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (NT > 64) {
+      __syncthreads();
+      if ((tid & 63) == 0) scratch[tid >> 6] = v;
+      __syncthreads();
+      v = scratch[0];
+#pragma unroll 1
+      for (int w = 1; w < NT / 64; ++w) v += scratch[w];
+      __syncthreads();
+    }
+    return v;
+  };
+  auto pass = [&](auto f) {  // f(logit, class); -inf past the row's end
+    for (int i = tid * V; i < K; i += STEP) {
+      Held<T> raw;
+      raw.load(z, i, K);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f(raw[e], i + e);
+    }
+  };
+  // the list; what is found of it: a class out of range, a class that may stand twice, the label's
+  constexpr int BAD = 1, TWICE = 2, LABEL = 4;
+  float mt = -__builtin_inff();
+  int found = 0;
+  int label = a.hard != 0.f ? a.y[row] : -1;
+  if (label >= K) found |= BAD, label = -1;
+  const int bits = Listed::bits(k, K);
+  for (int i = tid; i < bits / 32; i += NT) L.seen[i] = 0;
+  sync();
+  for (int j = tid; j < k; j += NT) {
+    int c = idx[j];
+    const float t = teacher_logit(a, row, j);
+    if (c < 0 || t == -__builtin_inff()) c = -1;
+    if (c >= K) found |= BAD, c = -1;
+    L.cls[j] = c, L.t[j] = t, L.z[j] = c < 0 ? 0.f : (float)z[c];
+    if (c < 0) continue;
+    mt = fmaxf(mt, t);
+    const uint32_t b = 1u << (c & 31);
+    if (atomicOr(&L.seen[(c & (bits - 1)) >> 5], b) & b) found |= TWICE;
+    if (c == label) found |= LABEL;
+  }
+  if (tid == 0) {
+    L.z[k] = label < 0 ? 0.f : (float)z[label];
+    for (int j = k; j < cap; ++j) L.cls[j] = j == k && label >= 0 ? label : -1, L.q[j] = 0.0;
+  }
+  mt = finite_max(block_reduce<NT>(mt, reinterpret_cast<float*>(scratch), fmax2));
+  found = block_reduce<NT>(found, reinterpret_cast<int*>(scratch), [](int x, int y) { return x | y; });
+  double S = 0.0;
+  for (int j = tid; j < k; j += NT) {
+    const double q = L.cls[j] < 0 ? 0.0 : exp(((double)L.t[j] - (double)mt) * rT);
+    L.q[j] = q;
+    S += q;
+  }
+  S = sum(S);
+  const double Q = (found & BAD) != 0 ? (double)__builtin_nanf("") : S == 0.0 ? 0.0 : S / S, H = label < 0 ? 0.0 : (double)a.hard;
+  // the row
+  RowStats r{-__builtin_inff(), 0.f, 0.f, 0};
+  pass([&](float x, int) { r.m = fmaxf(r.m, x); });
+  r.m = block_reduce<NT>(r.m, reinterpret_cast<float*>(scratch), fmax2);
+  const double m = finite_max(r.m);
+  double st = 0.0, s1 = 0.0;
+  int arg = K;
+  pass([&](float x, int i) {
+    const double d = (double)x - m;
+    st += exp(d * rT);
+    if (a.hard != 0.f) s1 += exp(d);
+    if (x == r.m) arg = min(arg, i);
+  });
+  st = sum(st), s1 = sum(s1);
+  arg = block_reduce<NT>(arg, reinterpret_cast<int*>(scratch), [](int x, int y) { return min(x, y); });
+  r.st = (float)st, r.s1 = (float)s1, r.arg = arg == K ? 0 : arg;
+  const bool none = st == 0.0;
+  if (a.loss != nullptr) {
+    double part = 0.0;
+    if (a.soft != 0.f && S != 0.0 && !none) {
+      const double ratio = log(st / S);
+      for (int j = tid; j < k; j += NT) {
+        if (L.cls[j] < 0) continue;
+        const double term = ((double)L.t[j] - (double)mt) * rT - ((double)L.z[j] - m) * rT + ratio;
+        part += L.z[j] == -__builtin_inff() ? (double)__builtin_inff() : L.q[j] / S * term;
+      }
+    }
+    double loss = sum(part) * (double)a.soft * (double)a.T * (double)a.T;
+    if (!none && H != 0.0) loss += H * (log(s1) - ((double)L.z[k] - m));
+    loss = none ? (Q != Q ? Q : 0.0) : loss + (Q - Q) + (st - st);
+    if (tid == 0) a.loss[row] = (float)loss;
+  }
+  if (tid == 0) {
+    if (a.stats_out != nullptr) a.stats_out[row] = r;
+    if (a.pred != nullptr) a.pred[row] = r.arg;
+  }
+  if (a.dz == nullptr) return;
+  const float g = a.g != nullptr ? a.g[row] : 1.f;
+  const double soft = (double)a.soft * (double)a.T;
+  sync();
+  for (int j = tid; j <= k; j += NT) {
+    const int c = L.cls[j];
+    // a class that stands once writes itself, and takes the label along
+    bool mine = c >= 0 && !(j == k && (found & LABEL) != 0);
+    double q = L.q[j], hit = c == label ? 1.0 : 0.0;
+    if ((found & TWICE) != 0) q = hit = 0.0;
+    for (int i = 0; mine && (found & TWICE) != 0 && i < cap; i += 4) {  // its first entry sums all of it, in their order
+      const int4 o = *reinterpret_cast<const int4*>(L.cls + i);
+      const int oc[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (oc[e] == c) {
+          if (i + e < j) mine = false;
+          if (i + e == k)
+            hit = 1.0;
+          else
+            q += L.q[i + e];
+        }
+    }
+    L.keep[j] = mine ? 1 : 0;
+    if (mine) {
+      const double d = (double)L.z[j] - m;
+      double v = none ? Q - Q : soft * (exp(d * rT) / st * Q - (S == 0.0 ? 0.0 : q / S));
+      if (!none && H != 0.0) v += H * (exp(d) / s1 - hit);
+      L.z[j] = (float)((double)g * v);
+    }
+  }
+  float at, a1;
+  dense_coeffs(a, g, (float)Q, (float)H, r, at, a1);
+  TO* dz = static_cast<TO*>(a.dz) + row * a.ldd;
+  sync();  // the listed logits have been read
+  stream_grad<T, TO, NT>(a, z, dz, 0, K, r, at, a1);
+  sync();
+  for (int j = tid; j <= k; j += NT)
+    if (L.keep[j] != 0) dz[L.cls[j]] = (TO)L.z[j];
+}
+
 // ---- host ---------------------------------------------------------------------------------------
+// Rows [r0, r0 + rows) of a call.
+template <class T, class TO>
+Args rows_from(const Args& a, int64_t r0, int64_t rows) {
+  Args b = a;
+  b.B = rows;
+  b.Z = static_cast<const T*>(a.Z) + r0 * a.ldz;
+  b.idx = a.idx + r0 * a.ldi;
+  b.t = static_cast<const char*>(a.t) + r0 * a.ldt * (int64_t)dtype_size(a.t_dt);
+  if (a.y) b.y = a.y + r0;
+  if (a.g) b.g = a.g + r0;
+  if (a.loss) b.loss = a.loss + r0;
+  if (a.pred) b.pred = a.pred + r0;
+  if (a.stats_in) b.stats_in = a.stats_in + r0;
+  if (a.stats_out) b.stats_out = a.stats_out + r0;
+  if (a.dz) b.dz = static_cast<TO*>(a.dz) + r0 * a.ldd;
+  return b;
+}
+
+// Few threads for short rows, of whose blocks a CU holds many.
+template <class T, class TO>
+void launch_hot(const Args& a, hipStream_t stream) {
+  constexpr int64_t MOST = 1 << 21;  // rows of a launch: a grid holds 2^32 threads
+  const size_t lds = HotListed::bytes(a.k, a.K);
+  for (int64_t r0 = 0; r0 < a.B; r0 += MOST) {
+    const Args b = rows_from<T, TO>(a, r0, std::min(MOST, a.B - r0));
+    const dim3 grid((unsigned)b.B);
+    if (a.K <= 2048)
+      hipLaunchKernelGGL((distill_hot_kernel<T, TO, 64>), grid, dim3(64), lds, stream, b);
+    else if (a.K <= 16384)
+      hipLaunchKernelGGL((distill_hot_kernel<T, TO, 256>), grid, dim3(256), lds, stream, b);
+    else
+      hipLaunchKernelGGL((distill_hot_kernel<T, TO, 1024>), grid, dim3(1024), lds, stream, b);
+    MLAPI_HIP_CHECK(hipGetLastError());
+  }
+}
+
 template <class T, class TO, int NTR, int NV>
 void launch_rows(const Args& a, hipStream_t stream) {
   constexpr int NT = NTR < 256 ? 256 : NTR, RPB = NT / NTR;
@@ -622,25 +844,15 @@ void launch_resident(const Args& a, hipStream_t stream) {
 
 template <class T, class TO>
 void run_distill(Args a, RowStats* ws, hipStream_t stream) {
+  if (a.T > HOT_T) return launch_hot<T, TO>(a, stream);
   const Plan p = make_plan<T>(a.B, a.K);
   if (p.parts == 0) return launch_resident<T, TO>(a, stream);
   const size_t lds = Listed::bytes(a.k, a.K);
   a.parts = 1;
   for (int64_t r0 = 0; r0 < a.B; r0 += 65535) {  // grid.y holds 16 bits
-    Args b = a;
     const unsigned rows = (unsigned)std::min<int64_t>(65535, a.B - r0);
-    b.Z = static_cast<const T*>(a.Z) + r0 * a.ldz;
-    b.idx = a.idx + r0 * a.ldi;
-    b.t = static_cast<const char*>(a.t) + r0 * a.ldt * (int64_t)dtype_size(a.t_dt);
-    if (a.y) b.y = a.y + r0;
-    if (a.g) b.g = a.g + r0;
-    if (a.loss) b.loss = a.loss + r0;
-    if (a.pred) b.pred = a.pred + r0;
-    if (a.stats_out) b.stats_out = a.stats_out + r0;
-    if (a.dz) b.dz = static_cast<TO*>(a.dz) + r0 * a.ldd;
-    if (a.stats_in) {
-      b.stats_in = a.stats_in + r0;
-    } else {
+    Args b = rows_from<T, TO>(a, r0, rows);
+    if (!a.stats_in) {
       hipLaunchKernelGGL((distill_parts_kernel<T>), dim3((unsigned)p.parts, rows), dim3(PART_THREADS), 0, stream, b,
                          p.len, ws + r0 * p.parts);
       b.stats_in = ws + r0 * p.parts;

@@ -197,6 +197,7 @@ def distill_loss(Z: torch.Tensor, idx: torch.Tensor, t: torch.Tensor, *, tempera
 
         loss = alpha T^2 sum_j q_j (ln q_j - ln p[idx_j])  -  (1 - alpha) ln softmax(Z)[y]        (f32 [B])
 
+    T in [1e-6, 1e6]; above 16, where T^2 would count what 32-bit sums are off, sums and loss are evaluated in 64 bits.
     A row without entries has no first part, a row with y < 0 no second, a row whose logits are all -inf
     neither. A listed class that the student masks makes the loss +inf. A class >= K in idx or y makes its
     row's loss and gradient NaN."""

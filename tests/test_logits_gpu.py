@@ -1,4 +1,5 @@
 """Row operators over class logits (top_logits, distill_*, sample_logits) against plain 64-bit forms."""
+import math
 import random
 
 import pytest
@@ -132,6 +133,86 @@ def test_distill_one_list_for_all_rows():
     loss, dz = ops.distill_loss_grad(Z, idx.expand(9, -1), t.expand(9, -1), temperature=2.0)
     l2, d2 = ops.distill_loss_grad(Z, idx.repeat(9, 1), t.repeat(9, 1), temperature=2.0)
     assert same(loss, l2) and same(dz, d2)
+
+
+def hot_bounds(Z, idx, t, loss, dz, *, temperature, alpha, y=None, g=None):
+    """Bounds at temperatures above 16, where sums, listed classes and the loss are 64-bit: both sides' exponentials (2
+    steps of 2^-52) and sums over at most 64 terms a thread, a wave's and a block's, count T^2 in the loss; the loss is rounded
+    to f32 once. A class that is not listed: an f32 exponential, its argument rounded three times, two factors. The
+    gradient is rounded to its type through f32."""
+    T, z, u, w = temperature, Z.double(), 2.0 ** -24, 2.0 ** -52
+    K = z.shape[1]
+    x = (z.masked_fill(z == INF, 0).amax(1, keepdim=True).clamp(min=-1e300) - z).nan_to_num(0.0, posinf=0.0)
+    live = (z > -INF).any(1, keepdim=True)
+    p, p1 = (torch.softmax(torch.where(live, z / s, torch.zeros_like(z)), 1) * live for s in (T, 1.0))
+    far = x.amax(1) / T  # the logarithms are at most this and ln K
+    tol_loss = 2 * u * loss.abs() + alpha * T * T * (100 * w + (math.log(K) + far) * 8 * w)
+    listed = torch.zeros(z.shape, dtype=torch.bool).scatter_(1, idx.long().clamp(0, K - 1), (idx >= 0) & (t > -INF))
+    tol_dz = alpha * T * (p + 1) * 100 * w + alpha * T * p * (3 * x / T + 8) * u * ~listed
+    if y is not None and alpha != 1.0:
+        tol_dz = tol_dz + (1 - alpha) * p1 * (3 * x + 8) * u
+    if g is not None:
+        tol_dz = tol_dz * g.double().abs()[:, None]
+    half = {torch.float32: u, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[Z.dtype]
+    tiny = torch.finfo(Z.dtype).tiny * (half if Z.dtype == torch.float16 else 2)
+    return tol_loss, tol_dz + (half + u) * dz.abs() + tiny
+
+
+@pytest.mark.parametrize("temperature", [16.0, 16.5, 100.0, 1e4, 1e6])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K,k", [(3, 2, 2), (5, 64, 64), (4, 1000, 1000), (6, 1024, 40), (3, 3000, 900), (2, 20000, 700),
+                                   (2, 140001, 900)])
+def test_distill_at_high_temperatures(B, K, k, dtype, temperature):
+    """Lists of every class that the student does not mask (and, k = 40, of some): p nears q, the loss does not vanish."""
+    hidden = torch.ones(K, dtype=torch.bool)
+    hidden[torch.randperm(K, generator=torch.Generator().manual_seed(1))[:max(k, 64)]] = False
+    Z = rows(B, K, torch.float32, 5)
+    t = Z + 0.7 * torch.randn(B, K, generator=torch.Generator().manual_seed(2))
+    Z = Z.masked_fill(hidden, -INF).to(dtype).to(DEV)
+    t, idx = ops.top_logits(t.masked_fill(hidden, -INF).to(dtype).to(DEV), k)
+    if k > 2:
+        idx[0, 1], t[0, 2] = idx[0, 0], -INF  # a class twice, an entry absent
+    for alpha in (1.0, 0.4):
+        y = g = None
+        if alpha != 1.0:
+            y = idx[:, min(k - 1, 7)].clone()
+            y[0] = -1
+            g = torch.linspace(-1, 2, B).to(DEV)
+        kw = dict(temperature=temperature, alpha=alpha, y=y)
+        rl, rd = ref.distill_ref(Z, idx, t, g=g, **kw)
+        cpu = lambda v: None if v is None else v.cpu()  # noqa: E731
+        how = dict(temperature=temperature, alpha=alpha, y=cpu(y), g=cpu(g))
+        bounds = hot_bounds if temperature > 16 else distill_bounds
+        tl, td = bounds(Z.cpu(), idx.cpu(), t.cpu(), rl.cpu(), rd.cpu(), **how)
+        if temperature == 1e4 and k == K and alpha == 1.0:
+            assert (tl <= 1e-4 * rl.cpu().abs() + 1e-5).all()  # the bound itself is far below the loss
+        loss, dz = ops.distill_loss_grad(Z, idx, t, g=g, **kw)
+        l2, stats = ops.distill_loss(Z, idx, t, **kw)
+        d2 = ops.distill_grad(Z, idx, t, stats, g=g, **kw)
+        own = Z.clone()
+        l3, d3 = ops.distill_loss_grad(own, idx, t, g=g, out=own, **kw)
+        assert temperature <= 16 or same(loss, l2) and same(dz, d2) and same(loss, l3) and same(dz, d3)
+        l, d, rl, rd = loss.double().cpu(), dz.double().cpu(), rl.cpu(), rd.cpu()
+        ok = (l - rl).abs() <= tl
+        assert ok.all(), (l[~ok], rl[~ok], tl[~ok])
+        ok = (d - rd).abs() <= td
+        assert ok.all(), (d[~ok][:4], rd[~ok][:4], td[~ok][:4], ok.logical_not().nonzero()[:4])
+
+
+def test_distill_at_high_temperatures_of_rows_without_a_class_or_out_of_range():
+    for K in (40, 5000, 40000):
+        Z = rows(8, K, torch.float32, 1, device=DEV)
+        idx, t = teacher(Z, 8, 1, device=DEV)
+        y = torch.zeros(8, dtype=torch.int32, device=DEV)
+        Z[0], Z[2, 5], Z[3, 7] = -INF, float("nan"), INF
+        idx[4, 2], y[5] = K, K + 9
+        t[6, 1] = float("nan")
+        Z[7, idx[7, 0].long()] = -INF
+        pred = torch.empty(8, dtype=torch.int32, device=DEV)
+        loss, dz = ops.distill_loss_grad(Z, idx, t, temperature=50.0, alpha=0.5, y=y, pred=pred)
+        assert loss[0] == 0 and (dz[0] == 0).all() and loss[2:7].isnan().all() and dz[2:7].isnan().all()
+        assert loss[1].isfinite() and dz[1].isfinite().all() and loss[7] == INF and dz[7].isfinite().all()
+        assert pred[1] == Z[1].argmax() and pred[3] == 7 and pred[0] == 0
 
 
 def test_distill_nan_inf_and_classes_out_of_range():
