@@ -210,7 +210,7 @@ def main(argv=None) -> int:
     p.add_argument("--kind", default="multinomial", choices=["multinomial", "ovr"])
     p.add_argument("--noise", type=float, default=1.0, help="multiclass synthetic label noise")
     p.add_argument("--graph", action="store_true", help="capture the single-GPU step in a HIP graph")
-    p.add_argument("--teacher", default="", help="checkpoint of the model to distil from (softmax, classes > 2)")
+    p.add_argument("--teacher", default="", help="checkpoint of the model to distil from (softmax or one-vs-rest, classes > 2)")
     p.add_argument("--teacher-top", type=int, default=16, help="teacher logits kept per row")
     p.add_argument("--temperature", type=float, default=2.0, help="of the distillation")
     p.add_argument("--alpha", type=float, default=0.5, help="weight of the teacher's targets; 1 - alpha: the labels'")

@@ -50,8 +50,9 @@ def synthetic_multiclass(n: int, F: int, K: int, *, seed: int = 0, device=None, 
 
 def teacher_top(model, X: torch.Tensor, k: int, *, rows: int = 1 << 16) -> Tuple[torch.Tensor, torch.Tensor]:
     """What a teacher (a :class:`~mlapi_amd.models.linear.LinearModel` of at least 3 classes) writes down for the rows of
-    X [n, F]: the classes (int32 [n, k]) and logits (f32 [n, k]) of its k largest logits, on X's device. On a GPU its
-    logits are bf16 products with f32 sums, ``rows`` rows at a time."""
+    X [n, F]: the classes (int32 [n, k]) and logits (f32 [n, k]) of its k largest logits, on X's device. Their softmax over
+    all classes is its ``predict_proba``: a one-vs-rest teacher's are ln sigmoid(z), in the order of z. On a GPU z is
+    bf16 products with f32 sums, ``rows`` rows at a time."""
     W, b = torch.as_tensor(model.W), torch.as_tensor(model.b)
     if W.shape[0] < 2 or W.shape[1] != X.shape[1]:
         raise ValueError(f"the teacher must have one row per class and {X.shape[1]} features (W is {tuple(W.shape)})")
@@ -61,7 +62,7 @@ def teacher_top(model, X: torch.Tensor, k: int, *, rows: int = 1 << 16) -> Tuple
         from mlapi_amd.ops.reference import top_logits_ref
 
         t, idx = top_logits_ref((X.double() @ W.T + b).float(), k)
-        return idx, t
+        return idx, torch.nn.functional.logsigmoid(t) if model.kind == Kind.OVR else t
     from mlapi_amd.ops.linear import gemm_logits
     from mlapi_amd.ops.logits import top_logits
 
@@ -71,7 +72,7 @@ def teacher_top(model, X: torch.Tensor, k: int, *, rows: int = 1 << 16) -> Tuple
     for s in range(0, X.shape[0], rows):
         Z = gemm_logits(X[s:s + rows].to(torch.bfloat16).contiguous(), W, b)
         top_logits(Z, k, out=(t[s:s + rows], idx[s:s + rows]))
-    return idx, t
+    return idx, torch.nn.functional.logsigmoid(t) if model.kind == Kind.OVR else t
 
 
 def _kernel_width(F: int) -> int:

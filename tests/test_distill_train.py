@@ -55,6 +55,30 @@ def test_trainer_refusals():
         teacher_top(LinearModel.random(4, 3, seed=0), X, 4)
 
 
+def _teacher_shares(kind, n, F, K, device):
+    """The softmax of a full-length list, by class, and the teacher's own probabilities; weights and features in bf16."""
+    g = torch.Generator().manual_seed(K)
+    W, X = (3 * torch.randn(s, F, generator=g).to(torch.bfloat16).float() / 4 for s in (K, n))
+    m = LinearModel(W.to(torch.bfloat16).double().numpy(), torch.randn(K, generator=g).numpy(), np.arange(K), kind)
+    X = X.to(torch.bfloat16).float()
+    idx, t = teacher_top(m, X.to(device), K, rows=16)
+    q = torch.zeros(n, K, dtype=torch.float64)
+    q.scatter_(1, idx.long().cpu(), torch.softmax(t.double().cpu(), 1))
+    # z: F + 1 products of at most 9 each (f32 sums), ln sigmoid two roundings of a number of its size; a softmax moves
+    # by at most twice what a logit does, relative
+    z = m.decision_function(X.numpy())
+    tol = 2 * ((F + 2) * 2.0 ** -24 * 9 * F ** 0.5 * 4 + 4 * 2.0 ** -24 * np.abs(z).max())
+    return q.numpy(), m.predict_proba(X.numpy()), tol, idx.cpu().numpy(), z
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("kind", [Kind.MULTINOMIAL, Kind.OVR])
+def test_a_teachers_list_has_its_probabilities(kind, device):
+    q, p, tol, idx, z = _teacher_shares(kind, 50, 40, 7, device)
+    assert (np.abs(q - p) <= tol * p + 1e-30).all()
+    assert (np.take_along_axis(z, idx.astype(np.int64), 1)[:, 0] >= z.max(1) - tol).all()
+
+
 def test_teacher_of_all_classes_and_temperature_one_gives_its_own_weights_no_gradient():
     """A student that equals its teacher has nothing to learn but what preparing the features in bf16 moved."""
     X, y = synthetic_multiclass(30, 6, 5, seed=2)
