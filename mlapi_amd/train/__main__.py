@@ -56,6 +56,8 @@ def cmd_fit(X, y, args) -> int:
 def cmd_sgd(args) -> int:
     import torch
 
+    if args.teacher and (args.classes <= 2 or args.kind != "multinomial"):
+        raise SystemExit("--teacher distils softmax models: --classes above 2 and --kind multinomial")
     if args.classes > 2:
         return cmd_sgd_multiclass(args)
 

@@ -112,6 +112,17 @@ def test_cli_distils_from_a_checkpoint(tmp_path):
     assert out["classes"] == 5 and np.isfinite(out["final_loss"])
 
 
+@pytest.mark.parametrize("how", [(), ("--classes", "2"), ("--classes", "5", "--kind", "ovr")])
+def test_cli_refuses_a_teacher_it_would_not_follow(tmp_path, how):
+    from mlapi_amd.ckpt.native import save_native
+
+    path = str(tmp_path / "teacher.safetensors")
+    save_native(path, LinearModel.random(12, 5, seed=3))
+    r = subprocess.run([sys.executable, "-m", "mlapi_amd.train", "sgd", "--features", "12", "--rows-per-rank", "64", "--batch",
+                        "64", "--steps", "1", "--teacher", path, *how], capture_output=True, text=True, cwd=ROOT, timeout=300)
+    assert r.returncode != 0 and "--teacher" in r.stderr and "Traceback" not in r.stderr
+
+
 # ---------------------------------------------------------------------------------------- answers
 @pytest.fixture(scope="module")
 def estimator():
