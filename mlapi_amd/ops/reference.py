@@ -103,6 +103,8 @@ def top_logits_ref(Z, k: int):
 
 def distill_ref(Z, idx, t, *, temperature: float = 1.0, alpha: float = 1.0, y=None, g=None, dtype=torch.float64):
     """Oracle of ops.logits.distill_*: (loss [B], dZ [B, K]); also the CPU path of the trainer's distillation."""
+    if alpha != 1.0 and y is None:
+        raise ValueError("distill_ref: alpha below 1 mixes in hard labels and needs y")
     z, T = Z.to(dtype), float(temperature)
     B, K = z.shape
     inf = float("inf")

@@ -253,14 +253,16 @@ class SoftmaxSGDTrainer:
                 d = self.mom
             self.params.sub_(self.lr * d)
 
-    def _check_teacher(self, teacher) -> None:
+    def _check_teacher(self, teacher, y) -> None:
         if teacher is not None and self.kind != Kind.MULTINOMIAL:
             raise ValueError("SoftmaxSGDTrainer: distillation is for softmax (MULTINOMIAL) models")
+        if teacher is not None and y is None and self.alpha != 1.0:
+            raise ValueError("SoftmaxSGDTrainer: alpha below 1 mixes in hard labels and needs y")
 
     def step(self, Xa: torch.Tensor, y: torch.Tensor, teacher=None) -> None:
         """One SGD step on this rank's shard (Xa from :meth:`prepare`, y int32 class indices). ``teacher``: (idx, t) of
         the same rows (:func:`teacher_top`) makes it a distillation step; y may then be None at alpha 1."""
-        self._check_teacher(teacher)
+        self._check_teacher(teacher, y)
         if self._graph is not None and self._graph[1] is Xa and self._graph[2] is y and self._graph[3] is teacher:
             self._graph[0].replay()
         elif self.on_gpu and (self._dp is not None or self.info.world == 1):
@@ -283,7 +285,7 @@ class SoftmaxSGDTrainer:
         Single replica only (the all-reduce stays outside graphs)."""
         if not self.on_gpu or self.info.world != 1:
             raise RuntimeError("graph capture: single-GPU replica only")
-        self._check_teacher(teacher)
+        self._check_teacher(teacher, y)
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         saved = (self.params.clone(), None if self.mom is None else self.mom.clone())

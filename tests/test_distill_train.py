@@ -55,6 +55,19 @@ def test_trainer_refusals():
         teacher_top(LinearModel.random(4, 3, seed=0), X, 4)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+def test_labels_that_a_step_mixes_in_are_asked_for(device):
+    X, y = synthetic_multiclass(8, 4, 3, device=torch.device(device))
+    top = teacher_top(LinearModel.random(4, 3, seed=0), X, 2)
+    tr = SoftmaxSGDTrainer(4, 3, device=torch.device(device), alpha=0.3)
+    Xa, before = tr.prepare(X), tr.params.clone()
+    with pytest.raises(ValueError, match="needs y"):
+        tr.step(Xa, None, teacher=top)
+    assert tr.steps == 0 and torch.equal(tr.params, before)
+    with pytest.raises(ValueError, match="needs y"):
+        ref.distill_ref(X[:, :3], *top, alpha=0.3)
+
+
 def _teacher_shares(kind, n, F, K, device):
     """The softmax of a full-length list, by class, and the teacher's own probabilities; weights and features in bf16."""
     g = torch.Generator().manual_seed(K)
