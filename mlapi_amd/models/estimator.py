@@ -169,16 +169,26 @@ class LogisticRegression:
         return self._m().classes[self.predict_max(X)[0]]
 
     def _class_logits(self, X):
-        import torch
-
-        return torch.as_tensor(self._m().class_logits(X), dtype=torch.float32, device=self._torch_device())
+        """f64 [n, n_classes]: what the classes are ordered by (the decision function), their logits."""
+        m = self._m()
+        z = m.decision_function(X)
+        L = m.logits_of(z)
+        if not np.isfinite(L.max(axis=1)).all():
+            raise ValueError("a row has no finite logits: its features are past the model's range")
+        return (z if m.kind == Kind.OVR else L), L
 
     def predict_top(self, X, k: int):
         """The k most likely classes of every row, likeliest first: (labels [n, k], f32 logits [n, k]; their softmax
-        over all classes is :meth:`predict_proba`). ``k`` is at most the number of classes."""
+        over all classes is :meth:`predict_proba`). ``k`` is at most the number of classes. As in :meth:`predict`, the
+        order is that of the f64 decision function, equal ones by class."""
+        import torch
+
         if not 1 <= int(k) <= self._m().n_classes:
             raise ValueError(f"k must be in [1, {self._m().n_classes}] (got {k})")
-        Z = self._class_logits(X)
+        order, L = self._class_logits(X)
+        with np.errstate(over="ignore"):
+            near = order.astype(np.float32)
+        Z = torch.as_tensor(near, device=self._torch_device())
         if Z.is_cuda:
             from mlapi_amd.ops.logits import top_logits
 
@@ -187,15 +197,27 @@ class LogisticRegression:
             from mlapi_amd.ops.reference import top_logits_ref
 
             v, i = top_logits_ref(Z, int(k))
-        return self._m().classes[i.cpu().numpy()], v.cpu().numpy()
+        v, i = v.cpu().numpy(), i.cpu().numpy().astype(np.int64)
+        # rows whose order 32 bits do not tell: logits that are equal in them, or past their range
+        redo = (v[:, 1:] == v[:, :-1]).any(1) | ((near == v[:, -1:]).sum(1) > 1) | (i < 0).any(1)
+        if redo.any():
+            i[redo] = np.argsort(-order[redo], axis=1, kind="stable")[:, :int(k)]
+        return self._m().classes[i], np.take_along_axis(L, i, 1).astype(np.float32)
 
     def sample(self, X, u=None, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
         """A class drawn for every row from its predicted distribution: (labels [n], their probability among the
         classes the filters keep). ``u``: one random number in [0, 1) per row (None: drawn with ``random_state``);
-        temperature and filters as in :func:`mlapi_amd.ops.logits.sample_logits`. Temperature 0 is :meth:`predict`."""
+        temperature and filters as in :func:`mlapi_amd.ops.logits.sample_logits`, on f32 logits. Temperature 0 is
+        :meth:`predict`."""
         import torch
 
-        Z = self._class_logits(X)
+        _, L = self._class_logits(X)
+        with np.errstate(over="ignore"):
+            far = ~np.isfinite(L.astype(np.float32).max(axis=1))
+        if far.any():  # past the range of f32: what counts is the distance to the row's maximum
+            L = L.copy()
+            L[far] -= L[far].max(1, keepdims=True)
+        Z = torch.as_tensor(L, dtype=torch.float32, device=self._torch_device())
         if u is None:
             u = np.random.default_rng(self.random_state).random(Z.shape[0])
         u = torch.as_tensor(np.asarray(u, dtype=np.float32), device=Z.device)
@@ -204,6 +226,8 @@ class LogisticRegression:
         kw = dict(temperature=float(temperature), top_k=int(top_k), top_p=float(top_p), min_p=float(min_p))
         if not (kw["temperature"] >= 0 and kw["top_k"] >= 0 and 0 <= kw["top_p"] <= 1 and 0 <= kw["min_p"] <= 1):
             raise ValueError(f"temperature and top_k must be >= 0, top_p and min_p in [0, 1] (got {kw})")
+        if kw["temperature"] == 0:
+            return self.predict(X), np.ones(Z.shape[0], dtype=np.float32)
         if Z.is_cuda:
             from mlapi_amd.ops.logits import sample_logits
 

@@ -148,7 +148,10 @@ class LinearModel:
     def class_logits(self, X) -> np.ndarray:
         """[n, n_classes] logits whose softmax is :meth:`predict_proba`, of every kind: z; [0, z] or [-z, z] of a binary
         model; ln sigmoid(z) of a one-vs-rest one."""
-        z = self.decision_function(X)
+        return self.logits_of(self.decision_function(X))
+
+    def logits_of(self, z: np.ndarray) -> np.ndarray:
+        """:meth:`class_logits` from the decision function's values."""
         if self.kind == Kind.BINARY:
             return np.stack([np.zeros_like(z), z], axis=1)
         if self.kind == Kind.BINARY_SOFTMAX:

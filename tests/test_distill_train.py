@@ -173,6 +173,36 @@ def test_estimator_samples_and_tops(estimator):
         estimator.predict_top(X, 7)
 
 
+def _of_logits(z, kind, device):
+    """An estimator that answers its features: z = X."""
+    K = len(z[0])
+    clf = LogisticRegression(device=device)
+    clf.model_ = LinearModel(np.eye(K), np.zeros(K), np.arange(K), kind)
+    return clf
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("kind", [Kind.MULTINOMIAL, Kind.OVR])
+def test_estimator_orders_logits_that_32_bits_do_not_tell_apart(kind, device):
+    """ln sigmoid vanishes above 104 in f32, logits of 1e39 are past it, and neighbours in f64 share one f32."""
+    X = np.array([[110.0, 120, -5, 0, 3, -7], [1, 1 + 1e-12, 1 + 2e-12, 1 - 1e-12, 1, 1], [2, 2, 2, 2, 2, 2],
+                  [1e39, 2e39, -1e39, -2e39, 0, 1], [800, 900, 700, 1000, -800, -900], [-2e39, -3e39, -1e39, -4e39, -1e39, -5e39],
+                  [0, -0.0, 0, -1, 1, 0]])
+    clf = _of_logits(X, kind, device)
+    want = np.argsort(-X, axis=1, kind="stable")
+    assert (clf.predict(X) == want[:, 0]).all()
+    label, prob = clf.sample(X, np.full(len(X), 0.7), temperature=0.0)
+    assert (label == want[:, 0]).all() and (prob == 1).all()
+    with np.errstate(over="ignore"):
+        for k in range(1, 7):
+            top, L = clf.predict_top(X, k)
+            assert (top == want[:, :k]).all(), k
+            assert (L == np.take_along_axis(clf.model_.class_logits(X), want[:, :k], 1).astype(np.float32)).all()
+    if kind == Kind.MULTINOMIAL:  # rows past f32 are drawn from all the same
+        label, prob = clf.sample(X[[3, 5]], np.array([0.5, 0.75]))
+        assert label.tolist() == [1, 4] and prob.tolist() == [1.0, 0.5]
+
+
 @pytest.mark.gpu
 def test_estimator_on_the_gpu_answers_as_on_the_cpu(estimator):
     X = np.random.default_rng(2).standard_normal((300, 7))
