@@ -370,6 +370,13 @@ void launch_sgd_update_2d(float* params, const float* grad, float* momentum_buf,
 // Workspaces need no initialisation and may differ from call to call.
 constexpr int LOGIT_MAX_CLASSES = 1 << 20;
 constexpr int LOGIT_MAX_TOP = 1024;
+// Rows of one launch, of B in all: a grid holds 2^32 threads in a dimension, and a row takes up to 1024. Larger
+// batches go in slices of nearly the same size, so that none is of few rows and cut otherwise than the whole.
+constexpr int64_t LOGIT_LAUNCH_ROWS = 1 << 21;
+inline int64_t logit_slice_rows(int64_t B) {
+  const int64_t n = (B + LOGIT_LAUNCH_ROWS - 1) / LOGIT_LAUNCH_ROWS;
+  return (B + n - 1) / n;
+}
 
 // The k first classes of every row: values [B, k] in Z's type, idx int32 [B, k]; past the last
 // unmasked class value = -inf, idx = -1.

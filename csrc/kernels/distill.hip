@@ -776,19 +776,15 @@ Args rows_from(const Args& a, int64_t r0, int64_t rows) {
 // Few threads for short rows, of whose blocks a CU holds many.
 template <class T, class TO>
 void launch_hot(const Args& a, hipStream_t stream) {
-  constexpr int64_t MOST = 1 << 21;  // rows of a launch: a grid holds 2^32 threads
   const size_t lds = HotListed::bytes(a.k, a.K);
-  for (int64_t r0 = 0; r0 < a.B; r0 += MOST) {
-    const Args b = rows_from<T, TO>(a, r0, std::min(MOST, a.B - r0));
-    const dim3 grid((unsigned)b.B);
-    if (a.K <= 2048)
-      hipLaunchKernelGGL((distill_hot_kernel<T, TO, 64>), grid, dim3(64), lds, stream, b);
-    else if (a.K <= 16384)
-      hipLaunchKernelGGL((distill_hot_kernel<T, TO, 256>), grid, dim3(256), lds, stream, b);
-    else
-      hipLaunchKernelGGL((distill_hot_kernel<T, TO, 1024>), grid, dim3(1024), lds, stream, b);
-    MLAPI_HIP_CHECK(hipGetLastError());
-  }
+  const dim3 grid((unsigned)a.B);
+  if (a.K <= 2048)
+    hipLaunchKernelGGL((distill_hot_kernel<T, TO, 64>), grid, dim3(64), lds, stream, a);
+  else if (a.K <= 16384)
+    hipLaunchKernelGGL((distill_hot_kernel<T, TO, 256>), grid, dim3(256), lds, stream, a);
+  else
+    hipLaunchKernelGGL((distill_hot_kernel<T, TO, 1024>), grid, dim3(1024), lds, stream, a);
+  MLAPI_HIP_CHECK(hipGetLastError());
 }
 
 template <class T, class TO, int NTR, int NV>
@@ -843,7 +839,7 @@ void launch_resident(const Args& a, hipStream_t stream) {
 }
 
 template <class T, class TO>
-void run_distill(Args a, RowStats* ws, hipStream_t stream) {
+void run_rows(Args a, RowStats* ws, hipStream_t stream) {
   if (a.T > HOT_T) return launch_hot<T, TO>(a, stream);
   const Plan p = make_plan<T>(a.B, a.K);
   if (p.parts == 0) return launch_resident<T, TO>(a, stream);
@@ -869,6 +865,12 @@ void run_distill(Args a, RowStats* ws, hipStream_t stream) {
                        dim3(PART_THREADS), lds, stream, b, p.len);
   }
   MLAPI_HIP_CHECK(hipGetLastError());
+}
+
+template <class T, class TO>
+void run_distill(const Args& a, RowStats* ws, hipStream_t stream) {
+  const int64_t step = logit_slice_rows(a.B);
+  for (int64_t r0 = 0; r0 < a.B; r0 += step) run_rows<T, TO>(rows_from<T, TO>(a, r0, std::min(step, a.B - r0)), ws, stream);
 }
 
 }  // namespace

@@ -767,13 +767,27 @@ void launch_sample(const SampleCall& c, hipStream_t stream) {
   if (c.ldz < c.K) throw std::invalid_argument("sample: row stride below K");
   if (c.B > 0x7fffffff) throw std::invalid_argument("sample: more than 2^31 rows");
   if (c.ws_bytes < sample_workspace(c)) throw std::invalid_argument("sample: workspace too small");
-  Call a;
-  static_cast<SampleCall&>(a) = c;
-  a.c_all = 1.4426950408889634074 / (double)std::min(c.temperature_all, 0x1.fffffep127f);
-  if (c.dt == DT_F32) return run_sample<float>(a, stream);
-  if (c.dt == DT_BF16) return run_sample<__bf16>(a, stream);
-  if (c.dt == DT_F16) return run_sample<_Float16>(a, stream);
-  throw std::invalid_argument("sample: logits f32, bf16 or f16");
+  if (c.dt != DT_F32 && c.dt != DT_BF16 && c.dt != DT_F16)
+    throw std::invalid_argument("sample: logits f32, bf16 or f16");
+  const int64_t step = logit_slice_rows(c.B);
+  for (int64_t r0 = 0; r0 < c.B; r0 += step) {
+    Call a;
+    static_cast<SampleCall&>(a) = c;
+    a.c_all = 1.4426950408889634074 / (double)std::min(c.temperature_all, 0x1.fffffep127f);
+    a.B = std::min(step, c.B - r0);
+    a.Z = static_cast<const char*>(c.Z) + r0 * c.ldz * (int64_t)dtype_size(c.dt);
+    a.u = c.u + r0, a.idx = c.idx + r0, a.prob = c.prob + r0;
+    if (c.temperature != nullptr) a.temperature = c.temperature + r0;
+    if (c.top_k != nullptr) a.top_k = c.top_k + r0;
+    if (c.top_p != nullptr) a.top_p = c.top_p + r0;
+    if (c.min_p != nullptr) a.min_p = c.min_p + r0;
+    if (c.dt == DT_F32)
+      run_sample<float>(a, stream);
+    else if (c.dt == DT_BF16)
+      run_sample<__bf16>(a, stream);
+    else
+      run_sample<_Float16>(a, stream);
+  }
 }
 
 }  // namespace mlapi

@@ -218,12 +218,20 @@ void launch_top_logits(int dt, const void* Z, int64_t ldz, int64_t B, int K, int
   if (ldz < K) throw std::invalid_argument("top_logits: row stride below K");
   if (B > 0x7fffffff) throw std::invalid_argument("top_logits: more than 2^31 rows");
   if (ws_bytes < top_logits_workspace(dt, B, K, k)) throw std::invalid_argument("top_logits: workspace too small");
-  const TopArgs a{Z, values, idx, B, ldz, K, k};
+  if (dt != DT_F32 && dt != DT_BF16 && dt != DT_F16)
+    throw std::invalid_argument("top_logits: logits f32, bf16 or f16");
   uint64_t* lists = static_cast<uint64_t*>(workspace);
-  if (dt == DT_F32) return run_top<float>(a, lists, stream);
-  if (dt == DT_BF16) return run_top<__bf16>(a, lists, stream);
-  if (dt == DT_F16) return run_top<_Float16>(a, lists, stream);
-  throw std::invalid_argument("top_logits: logits f32, bf16 or f16");
+  const int64_t step = logit_slice_rows(B), size = (int64_t)dtype_size(dt);
+  for (int64_t r0 = 0; r0 < B; r0 += step) {
+    const TopArgs a{static_cast<const char*>(Z) + r0 * ldz * size, static_cast<char*>(values) + r0 * k * size, idx + r0 * k,
+                    std::min(step, B - r0), ldz, K, k};
+    if (dt == DT_F32)
+      run_top<float>(a, lists, stream);
+    else if (dt == DT_BF16)
+      run_top<__bf16>(a, lists, stream);
+    else
+      run_top<_Float16>(a, lists, stream);
+  }
 }
 
 }  // namespace mlapi

@@ -517,6 +517,32 @@ def test_many_short_rows():
     assert ((dz.double() - rd).abs() <= rd.abs() * 2.0 ** -11 + 200 * 2.0 ** -24 * 8 + 2.0 ** -25).all()
 
 
+def test_more_rows_than_a_launch_holds_threads_for():
+    """A wave to a row: 2^26 rows are 2^32 threads. The same 4099 rows again and again give the same again and again."""
+    n, times, K = 4099, 16373, 2
+    base = rows(n, K, torch.float16, 4, "bell", device=DEV)
+    Z = base.repeat(times, 1)
+    assert Z.shape[0] > 1 << 26
+    again = lambda v, one: same(v[:n], one) and torch.equal(v.view(times, *one.shape), one.expand(times, *one.shape))  # noqa: E731
+    val, idx = ops.top_logits(base, 2)
+    V, I = ops.top_logits(Z, 2)
+    assert again(V, val) and again(I, idx)
+    for T in (1.5, 20.0):
+        loss, dz = ops.distill_loss_grad(base, idx, val, temperature=T)
+        L, D = ops.distill_loss_grad(Z, I, V, temperature=T)
+        assert again(L, loss) and again(D, dz)
+        L, stats = ops.distill_loss(Z, I, V, temperature=T)
+        assert again(L, loss) and again(ops.distill_grad(Z, I, V, stats, temperature=T), dz)
+    del V, I, L, D, stats
+    u = torch.rand(n, generator=torch.Generator().manual_seed(1)).to(DEV)
+    k = torch.randint(0, 3, (n,), generator=torch.Generator().manual_seed(2)).to(torch.int32).to(DEV)
+    for f, F in ((dict(), dict()), (dict(top_k=k, top_p=0.6, temperature=1 + u, min_p=u),
+                                    dict(top_k=k.repeat(times), top_p=0.6, temperature=(1 + u).repeat(times), min_p=u.repeat(times)))):
+        idx, prob = ops.sample_logits(base, u, **f)
+        I, P = ops.sample_logits(Z, u.repeat(times), **F)
+        assert again(I, idx) and again(P, prob)
+
+
 def test_more_long_rows_than_a_grid_dimension():
     """Rows that are cut into parts, past 65535 of them (17 GB, written in place)."""
     B, K = 65539, 131077
