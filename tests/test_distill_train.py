@@ -277,6 +277,40 @@ def test_trainer_steps_on_the_gpu_follow_the_cpu_ones_and_a_captured_step_the_ea
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("momentum", [0.0, 0.9])
+def test_every_trainer_step_on_the_gpu_is_the_plain_one(momentum):
+    """Each step against 64 bits from the weights, shadows and momenta before it, to a bound that the step is far above."""
+    dev, u = torch.device("cuda", 0), 2.0 ** -24
+    n, F, K, k = 640, 60, 23, 6
+    lr, l2, T, alpha = 0.3, 1e-3, 1.5, 0.5
+    X, y = synthetic_multiclass(n, F, K, seed=3, device=dev)
+    top = teacher_top(LinearModel.random(F, K, seed=9), X, k)
+    tr = SoftmaxSGDTrainer(F, K, device=dev, lr=lr, l2=l2, momentum=momentum, temperature=T, alpha=alpha)
+    Xa = tr.prepare(X)
+    for _ in range(4):
+        before, mom = tr.params.double(), 0.0 if tr.mom is None else tr.mom.double()
+        zeros = torch.zeros(K, tr.F_aug - tr.Fk - 1, dtype=torch.float64, device=dev)
+        Wa = torch.cat([tr.shadow_w.double(), tr.shadow_b.double()[:, None], zeros], 1)
+        G, dW, loss, correct = ref.softmax_distill_ref(Xa, Wa, *top, temperature=T, alpha=alpha, y=y, dtype=torch.float64)
+        grad = dW / n
+        grad[:, :tr.Fk] += l2 * before[:, :tr.Fk]
+        want_mom = momentum * mom + grad
+        tr.step(Xa, y, teacher=top)
+        # as for the gradient alone: logits of Fk + 1 products, a row's sums, G once to bf16, a sum over n rows; then a
+        # mean, a decay, a momentum and a step of five roundings each at most
+        ez = (tr.Fk + 2) * u * (Xa.double().abs() @ Wa.abs().T).max()
+        eG = G.abs() * 2.0 ** -8 + 2 * ez + 1000 * u * T
+        e = (eG.T @ Xa.double().abs() + (n + 64) * u * (G.abs().T @ Xa.double().abs())) / n
+        tol = lr * e + 5 * u * (before.abs() + lr * (want_mom.abs() + grad.abs() + abs(momentum * mom))) + 1e-30
+        step = tr.params.double() - before
+        assert ((step + lr * want_mom).abs() <= tol).all(), ((step + lr * want_mom).abs() - tol).max()
+        assert step[:, :F + 1].abs().max() >= 30 * tol.max()
+        assert torch.equal(tr.shadow_w, tr.params[:, :tr.Fk].to(torch.bfloat16)) and torch.equal(tr.shadow_b, tr.b)
+        assert abs(tr.last_loss() - loss.item() / n) <= T * T * (2 * ez.item() + 1000 * u) * 4
+    assert tr.last_accuracy() == pytest.approx(correct.item() / n, abs=2 / n)
+
+
+@pytest.mark.gpu
 def test_teacher_student_answer_run():
     """The run as it is used: the teacher's top logits, the student's steps, its drawn answers."""
     dev = torch.device("cuda", 0)

@@ -126,6 +126,30 @@ def test_distill_longest_lists(B, K):
         check_distill(Z, idx, t, 1.5, 0.6, y)
 
 
+@pytest.mark.parametrize("dtype,B,K", [(torch.float32, 33, 33001), (torch.float32, 40, 65536), (torch.float32, 35, 32769)] +
+                         [(t, B, K) for t in TYPES[1:] for B, K in ((33, 65537), (40, 131072), (34, 131071))])
+def test_distill_longest_rows_in_registers(dtype, B, K):
+    """1024 threads of 16 vectors each: more than 32 rows of 8193 to 16384 vectors."""
+    k = 12
+    Z = rows(B, K, dtype, 9, "bell", pad=3, device=DEV)
+    idx, t = teacher(Z, k, 3, device=DEV)
+    idx[4, 0], idx[5, 1] = K - 1, 0
+    g = torch.linspace(-1, 1, B).to(DEV)
+    y = torch.randint(-1, K, (B,), generator=torch.Generator().manual_seed(K)).to(torch.int32).to(DEV)
+    y[4], y[6] = K - 1, idx[6, 2]
+    for kw in (dict(temperature=2.0, alpha=1.0), dict(temperature=1.0, alpha=0.5, y=y, g=g),
+               dict(temperature=0.7, alpha=0.4, y=y, g=g)):
+        loss, dz = check_distill(Z, idx, t, **kw)
+        pred = torch.empty(B, dtype=torch.int32, device=DEV)
+        own = Z.clone()  # the row stride of the clone: K
+        l2, d2 = ops.distill_loss_grad(own, idx, t, out=own, pred=pred, **kw)
+        assert d2.data_ptr() == own.data_ptr() and same(l2, loss) and same(d2, dz)
+        assert torch.equal(pred.long(), Z.float().argmax(1))
+        if dtype == torch.float32:
+            _, d3 = ops.distill_loss_grad(Z, idx, t, out=torch.empty(B, K, dtype=torch.bfloat16, device=DEV), **kw)
+            assert same(d3, dz.to(torch.bfloat16))
+
+
 def test_distill_one_list_for_all_rows():
     """idx and t may be expanded: a row stride of 0."""
     Z = rows(9, 700, torch.bfloat16, 2, "bell", device=DEV)
