@@ -311,6 +311,27 @@ def test_every_trainer_step_on_the_gpu_is_the_plain_one(momentum):
 
 
 @pytest.mark.gpu
+def test_two_ranks_on_the_gpu_distil_as_one(tmp_path):
+    """Two ranks that share the GPU: exchange inside the step's last kernel, apart from it, and by owner ranks."""
+    from test_comm_gpu import _torchrun
+
+    _torchrun(1, "distill_train_gpu.py", tmp_path)
+    for env in ({}, {"MLAPI_DP_FUSED": "0"}, {"MLAPI_DP_TWO_SHOT": "1"}):
+        _torchrun(2, "distill_train_gpu.py", tmp_path, env=env)
+    one = np.load(tmp_path / "params_1_0.npy")
+    ranks = [np.load(tmp_path / f"params_2_{r}{how}.npy") for how in ("", "_apart", "_two") for r in (0, 1)]
+    assert all(np.array_equal(ranks[0], v) for v in ranks[1:])
+    # G is the same to the bit in the first step; then a sum of n products (|G| <= T, features below 8) in another order, 64
+    # roundings of 2^-24 each way, moves a weight by lr times its mean, may move its bf16 shadow by a step, 2^-8 of it,
+    # and a logit by as much of 60^0.5 features: the next steps' gradients follow by T times that, momenta by 2
+    w = np.abs(one).max()
+    tol = 4 * 2 * 0.3 * (2 * 64 * 2.0 ** -24 * 2 * 8 + 2.0 ** -8 * w * 2)
+    assert np.abs(ranks[0] - one).max() <= tol and w >= 4 * tol
+    # a logit by 2^-8 w for each of 60 features of mean size below 1, and the loss by at most a T + 1 - a of it
+    assert abs(np.load(tmp_path / "loss_2_0.npy") - np.load(tmp_path / "loss_1_0.npy")) <= 1.6 * 60 * 2.0 ** -8 * w
+
+
+@pytest.mark.gpu
 def test_teacher_student_answer_run():
     """The run as it is used: the teacher's top logits, the student's steps, its drawn answers."""
     dev = torch.device("cuda", 0)
