@@ -263,7 +263,8 @@ class SoftmaxSGDTrainer:
         """One SGD step on this rank's shard (Xa from :meth:`prepare`, y int32 class indices). ``teacher``: (idx, t) of
         the same rows (:func:`teacher_top`) makes it a distillation step; y may then be None at alpha 1."""
         self._check_teacher(teacher, y)
-        if self._graph is not None and self._graph[1] is Xa and self._graph[2] is y and self._graph[3] is teacher:
+        if self._graph is not None and self._graph[1] is Xa and self._graph[2] is y and self._graph[3] is teacher and \
+                (teacher is None or self._graph[4] == (self.temperature, self.alpha)):
             self._graph[0].replay()
         elif self.on_gpu and (self._dp is not None or self.info.world == 1):
             self._local_grad(Xa, y, fused_update_n=Xa.shape[0] * self.info.world, dp=self._dp, teacher=teacher)
@@ -281,7 +282,8 @@ class SoftmaxSGDTrainer:
     def capture(self, Xa: torch.Tensor, y: torch.Tensor, teacher=None) -> None:
         """Capture one whole step (row stats + fused gradient + slab sums + update) in a HIP graph.
 
-        Later ``step(Xa, y, teacher)`` calls with these exact objects replay it: one launch from the host.
+        Later ``step(Xa, y, teacher)`` calls with these exact objects (and, with a teacher, the same temperature and
+        alpha) replay it: one launch from the host.
         Single replica only (the all-reduce stays outside graphs)."""
         if not self.on_gpu or self.info.world != 1:
             raise RuntimeError("graph capture: single-GPU replica only")
@@ -300,7 +302,7 @@ class SoftmaxSGDTrainer:
         self._refresh_shadow()
         if self.mom is not None:
             self.mom.copy_(saved[1])
-        self._graph = (g, Xa, y, teacher)
+        self._graph = (g, Xa, y, teacher, (self.temperature, self.alpha))
 
     # ---------------------------------------------------------------------------------- stats
     def last_loss(self) -> float:

@@ -311,6 +311,22 @@ def test_every_trainer_step_on_the_gpu_is_the_plain_one(momentum):
 
 
 @pytest.mark.gpu
+def test_a_captured_step_follows_the_temperature_and_alpha_of_the_moment():
+    dev = torch.device("cuda", 0)
+    X, y = synthetic_multiclass(300, 20, 5, seed=3, device=dev)
+    top = teacher_top(LinearModel.random(20, 5, seed=9), X, 4)
+    eager, graphed = (SoftmaxSGDTrainer(20, 5, device=dev, lr=0.3, temperature=2.0, alpha=0.5) for _ in range(2))
+    Xa = eager.prepare(X)
+    graphed.capture(Xa, y, top)
+    for T, alpha in ((2.0, 0.5), (5.0, 0.5), (5.0, 0.9), (2.0, 0.5)):
+        for tr in (eager, graphed):
+            tr.temperature, tr.alpha = T, alpha
+            tr.step(Xa, y, teacher=top)
+        torch.cuda.synchronize()
+        assert torch.equal(eager.params, graphed.params) and eager.last_loss() == graphed.last_loss(), (T, alpha)
+
+
+@pytest.mark.gpu
 def test_two_ranks_on_the_gpu_distil_as_one(tmp_path):
     """Two ranks that share the GPU: exchange inside the step's last kernel, apart from it, and by owner ranks."""
     from test_comm_gpu import _torchrun
