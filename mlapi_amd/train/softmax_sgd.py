@@ -253,16 +253,22 @@ class SoftmaxSGDTrainer:
                 d = self.mom
             self.params.sub_(self.lr * d)
 
-    def _check_teacher(self, teacher, y) -> None:
-        if teacher is not None and self.kind != Kind.MULTINOMIAL:
+    def _check_teacher(self, teacher, Xa, y) -> None:
+        if teacher is None:
+            return
+        if self.kind != Kind.MULTINOMIAL:
             raise ValueError("SoftmaxSGDTrainer: distillation is for softmax (MULTINOMIAL) models")
-        if teacher is not None and y is None and self.alpha != 1.0:
+        if y is None and self.alpha != 1.0:
             raise ValueError("SoftmaxSGDTrainer: alpha below 1 mixes in hard labels and needs y")
+        idx, t = teacher
+        if idx.dim() != 2 or idx.shape != t.shape or idx.shape[0] != Xa.shape[0]:
+            raise ValueError(f"SoftmaxSGDTrainer: a teacher's idx and t must be [{Xa.shape[0]}, k], a list for each row of "
+                             f"the batch (got {tuple(idx.shape)} and {tuple(t.shape)})")
 
     def step(self, Xa: torch.Tensor, y: torch.Tensor, teacher=None) -> None:
         """One SGD step on this rank's shard (Xa from :meth:`prepare`, y int32 class indices). ``teacher``: (idx, t) of
         the same rows (:func:`teacher_top`) makes it a distillation step; y may then be None at alpha 1."""
-        self._check_teacher(teacher, y)
+        self._check_teacher(teacher, Xa, y)
         if self._graph is not None and self._graph[1] is Xa and self._graph[2] is y and self._graph[3] is teacher and \
                 (teacher is None or self._graph[4] == (self.temperature, self.alpha)):
             self._graph[0].replay()
@@ -287,7 +293,7 @@ class SoftmaxSGDTrainer:
         Single replica only (the all-reduce stays outside graphs)."""
         if not self.on_gpu or self.info.world != 1:
             raise RuntimeError("graph capture: single-GPU replica only")
-        self._check_teacher(teacher, y)
+        self._check_teacher(teacher, Xa, y)
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         saved = (self.params.clone(), None if self.mom is None else self.mom.clone())

@@ -68,6 +68,18 @@ def test_labels_that_a_step_mixes_in_are_asked_for(device):
         ref.distill_ref(X[:, :3], *top, alpha=0.3)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+def test_a_teachers_lists_are_as_many_as_the_rows(device):
+    X, y = synthetic_multiclass(8, 4, 3, device=torch.device(device))
+    idx, t = teacher_top(LinearModel.random(4, 3, seed=0), X, 2)
+    tr = SoftmaxSGDTrainer(4, 3, device=torch.device(device), alpha=0.3)
+    Xa, before = tr.prepare(X), tr.params.clone()
+    for bad in ((idx[:1], t[:1]), (idx[:7], t[:7]), (idx, t[:, :1]), (idx[0], t[0]), (idx[:1], t)):
+        with pytest.raises(ValueError, match="a list for each row"):
+            tr.step(Xa, y, teacher=bad)
+    assert torch.equal(tr.params, before)
+
+
 def _teacher_shares(kind, n, F, K, device):
     """The softmax of a full-length list, by class, and the teacher's own probabilities; weights and features in bf16."""
     g = torch.Generator().manual_seed(K)
