@@ -15,8 +15,8 @@
 // class sums all entries of it, in their order: a class listed twice costs no atomic.
 //
 // Bound by memory where one softmax is asked for (a row is read once and written once, 7 operations per
-// logit): 65536 x 1000 f32 with labels, loss and gradient 108 us, 4.9 TB/s; 2048 x 65536 bf16 117 us, 4.6 TB/s,
-// the loss alone 52 us. By the exponentials where labels at another temperature add a second softmax to
+// logit): 65536 x 1000 f32 with labels, loss and gradient 108 us, 4.9 TB/s; 2048 x 65536 bf16 112 us, 4.8 TB/s;
+// loss and gradient apart 78 and 97 us. By the exponentials where labels at another temperature add a second softmax to
 // 16-bit logits: 1501 x 32003 f16 61 us, 3.2 TB/s.
 #include <hip/hip_runtime.h>
 

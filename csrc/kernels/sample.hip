@@ -19,8 +19,8 @@
 //   rows of up to 2048 classes: one wave, from registers (sample_wave_kernel);
 //   longer rows with a short top-k: the k first classes by one pass (row_top.h), few long rows in parts;
 //   longer rows else: one block, from memory, a pass of weights and one of those kept (sample_row_kernel).
-// Bound by the issue of the weights' f64 instructions, 26 per logit: 65536 x 1000 f32 without filters 79 us (85 % of
-// it issue), p = 0.9: 175 us, k = 50: 150 us; 256 x 65537 bf16, p = 0.9: 65 us. By two launches where few rows
+// Bound by the issue of the weights' f64 instructions, 26 per logit: 65536 x 1000 f32 without filters 78 to 84 us (85 %
+// of it issue), p = 0.9: 181 us, k = 50: 149 us; 256 x 65537 bf16, p = 0.9: 66 to 70 us. By two launches where few rows
 // have a short top-k: 1 x 131072 f32, k = 50: 16 us.
 #include <hip/hip_runtime.h>
 

@@ -5,11 +5,11 @@ Each takes logits ``Z`` [B, K] (f32, bf16 or f16; B rows of one sample's K class
 stride, and launches on the current stream of Z's device. They allocate their results and workspace from
 torch's allocator and do not synchronise, so they can be captured into a HIP graph. GPU tensors only;
 plain oracles are in :mod:`mlapi_amd.ops.reference`. Gradients are results like any other: nothing here is recorded by
-autograd.
+autograd (``Z.backward(dZ)`` hands them on to the model that gave Z).
 
 The order of a row's classes is everywhere: larger logit first, then lower class. A class whose logit is
 -inf is masked; so is NaN in :func:`top_logits` and :func:`sample_logits`, while in the distillation loss a
-NaN makes its row NaN.
+NaN or +inf makes its row NaN.
 
     values, idx = top_logits(teacher_Z, 16)                               # the teacher's list
     loss, dZ = distill_loss_grad(student_Z, idx, values, temperature=2.0)  # the student's step
