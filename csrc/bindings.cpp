@@ -444,7 +444,8 @@ PYBIND11_MODULE(_C, m) {
       },
       py::arg("dt"), py::arg("Z"), py::arg("ldz"), py::arg("B"), py::arg("K"), py::arg("k"), py::arg("values"),
       py::arg("idx"), py::arg("ws"), py::arg("ws_bytes"), py::arg("stream") = 0);
-  m.def("distill_workspace", &distill_workspace, py::arg("dt"), py::arg("B"), py::arg("K"));
+  m.def("distill_workspace", &distill_workspace, py::arg("dt"), py::arg("B"), py::arg("K"),
+        py::arg("temperature") = 1.f, py::arg("stats_given") = false);
   m.def(
       "distill",
       [](int dt, int t_dt, int out_dt, uintptr_t Z, int64_t ldz, int64_t B, int K, uintptr_t idx, int64_t ldi,

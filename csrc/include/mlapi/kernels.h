@@ -388,7 +388,7 @@ void launch_top_logits(int dt, const void* Z, int64_t ldz, int64_t B, int K, int
 // with row strides; y int32 [B] or null; g f32 [B] or null (1). Any of loss f32 [B], stats_out
 // (16 bytes per row), pred int32 [B] (first maximum), dz [B, K] may be null. With stats_in (an
 // earlier call's stats_out on the same Z, temperature and alpha) the row sums are not computed again, but
-// above a temperature of 16, where they take 64 bits.
+// for rows that take 64 bits (above a temperature of 16).
 struct DistillCall {
   int dt = 0, t_dt = 0, out_dt = 0;
   const void* Z = nullptr;
@@ -407,7 +407,7 @@ struct DistillCall {
   void* workspace = nullptr;
   size_t ws_bytes = 0;
 };
-size_t distill_workspace(int dt, int64_t B, int K);
+size_t distill_workspace(int dt, int64_t B, int K, float temperature = 1.f, bool stats_given = false);
 void launch_distill(const DistillCall& call, hipStream_t stream);
 
 // Distillation step of the multiclass trainer (softmax_distill.hip): logits of X_aug (its first F columns)

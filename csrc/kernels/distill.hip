@@ -52,8 +52,10 @@ struct Args {
   RowStats* stats_out;
   void* dz;
   int32_t* pred;
+  int32_t* near;  // [B] or null: whether a row takes 64 bits (below)
   int64_t B, ldz, ldi, ldt, ldd;
   int K, k, parts, t_dt;
+  bool find;  // near is written by this launch, else read
   float T, soft, hard;  // soft = a, hard = 1 - a (0 without labels)
   bool two;             // labels at a temperature other than the teacher's: a second softmax
 };
@@ -188,6 +190,17 @@ __device__ float row_loss(const Args& a, int lane, Listed L, float S, float Q, f
   return loss + (Q - Q) + (r.st - r.st);
 }
 
+// Whether p and q are near each other throughout (one wave, L as read_listed gave it): all but 1/64 of p lies on the
+// listed classes. Otherwise the loss is at least T^2 / 64 of its soft part, and sums 2^-22 off show as 2^-16 of it.
+__device__ bool near_rows(const Args& a, int lane, Listed L, float S, RowStats r) {
+  if (a.soft == 0.f || S == 0.f || r.st == 0.f) return false;
+  const float ct = 1.44269504088896340736f / a.T, m = finite_max(r.m);
+  float on = 0.f;
+  for (int j = lane; j < a.k; j += 64)
+    if (L.cls[j] >= 0) on += __builtin_amdgcn_exp2f((L.z[j] - m) * ct);
+  return wave_sum(on) > r.st * (63.f / 64.f);
+}
+
 // Coefficients of the dense part: dz_i = at exp((z_i - m) / T) + a1 exp(z_i - m).
 __device__ __forceinline__ void dense_coeffs(const Args& a, float g, float Q, float H, RowStats r, float& at,
                                              float& a1) {
@@ -256,7 +269,7 @@ template <class T, class TO, int NTR, int NV>
 __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill_rows_kernel(Args a) {
   constexpr int V = Vec<T>::N, NT = NTR < 256 ? 256 : NTR, RPB = NT / NTR;
   __shared__ float scratch[NT / 64];
-  __shared__ float bcast[RPB][2];
+  __shared__ float bcast[RPB][3];
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int sub = RPB == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / NTR);
   const int tid = RPB == 1 ? (int)threadIdx.x : (int)threadIdx.x % NTR, lane = threadIdx.x & 63;
@@ -335,8 +348,15 @@ __global__ __launch_bounds__(NTR < 256 ? 256 : NTR, NV > 8 ? 4 : 8) void distill
     arg = block_reduce<NTR>(arg, reinterpret_cast<int*>(scratch), [](int x, int y) { return min(x, y); });
     r.arg = arg == K ? 0 : arg;
   }
+  bool near = false;
+  if (a.near != nullptr && tid < 64) {
+    near = near_rows(a, lane, L, S, r);
+    if (lane == 0) a.near[row] = near ? 1 : 0;
+    if (NTR > 64 && lane == 0) bcast[sub][2] = near ? 1.f : 0.f;
+  }
   sync();
-  if (NTR > 64) Q = bcast[sub][0], H = bcast[sub][1];
+  if (NTR > 64) Q = bcast[sub][0], H = bcast[sub][1], near = a.near != nullptr && bcast[sub][2] != 0.f;
+  if (near) return;  // all threads of the row: its results are distill_hot_kernel's
   const float g = a.g != nullptr ? a.g[row] : 1.f;
   float at, a1;
   dense_coeffs(a, g, Q, H, r, at, a1);
@@ -524,6 +544,7 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
   __shared__ float bcast[2];
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int64_t row = blockIdx.y;
+  if (a.near != nullptr && !a.find && a.near[row] != 0) return;  // its results are distill_hot_kernel's
   const int lane = threadIdx.x & 63, cap = Listed::capacity(a.k);
   const float ct = 1.44269504088896340736f / a.T, ce = 1.44269504088896340736f;
   Listed L(dyn, cap);
@@ -547,6 +568,11 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
     dense_coeffs(a, g, Q, H, r, at, a1);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
+    if (a.near != nullptr && a.find) {  // one block to a row, no gradient
+      const bool near = near_rows(a, lane, L, S, r);
+      if (lane == 0) a.near[row] = near ? 1 : 0;
+      if (near) return;
+    }
     if (blockIdx.x == 0) {
       if (a.loss != nullptr) {
         const float loss = row_loss(a, lane, L, S, Q, H, r);
@@ -574,10 +600,11 @@ __global__ __launch_bounds__(PART_THREADS) void distill_chunks_kernel(Args a, in
 // ---- high temperatures --------------------------------------------------------------------------
 // A list of every class leaves p and q only (z - t) / T apart, while the loss, T^2 times a difference of their
 // logarithms, stays of the size of (z - t)^2: what an f32 sum is off, about 2^-22, counts T^2 times (6e-5 at T = 16),
-// and T times in the gradient of a listed class. Above, the sums, the listed classes and the loss are evaluated in
-// 64 bits, T^2 2^-50; the dense part, where nothing cancels, is not. One block to a row, which it reads three times, the
-// last two from the caches where it is not too long; bound by 64-bit exponentials, one a logit (two with labels).
-// 65536 x 1000 f32 with labels: 257 us, 108 at T <= 16; 2048 x 65536 bf16: 353 and 114; 7 x 200001 f32: 87 and 16.
+// and T times in the gradient of a listed class. Above, rows whose list holds nearly all of p (near_rows) are left out by
+// the launches before, and their sums, listed classes and loss evaluated in 64 bits, T^2 2^-50; the dense part, where
+// nothing cancels, is not. One block to a row, which it reads three times, the last two from the caches where it is not
+// too long; bound by 64-bit exponentials, one a logit (two with labels). 256 x 1000 f32, all 1000 listed: 36 us, 18 at
+// T = 16; 65536 x 1000 f32 of 16 listed, no row near: 127 us, 111 at T = 16; 7 x 200001 f32 of 33: 21 us, 15.
 constexpr float HOT_T = 16.f;
 
 // The listed classes of one row, in LDS: n = k entries, and the label as one more.
@@ -606,6 +633,7 @@ __global__ __launch_bounds__(NT) void distill_hot_kernel(Args a) {
   __shared__ double scratch[NT / 64];
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int64_t row = blockIdx.x;
+  if (a.near[row] == 0) return;
   const int K = a.K, k = a.k, tid = threadIdx.x, cap = Listed::capacity(k);
   const double rT = 1.0 / (double)a.T;
   const T* z = static_cast<const T*>(a.Z) + row * a.ldz;
@@ -667,6 +695,7 @@ __global__ __launch_bounds__(NT) void distill_hot_kernel(Args a) {
     L.z[k] = label < 0 ? 0.f : (float)z[label];
     for (int j = k; j < cap; ++j) L.cls[j] = j == k && label >= 0 ? label : -1, L.q[j] = 0.0;
   }
+  sync();
   mt = finite_max(block_reduce<NT>(mt, reinterpret_cast<float*>(scratch), fmax2));
   found = block_reduce<NT>(found, reinterpret_cast<int*>(scratch), [](int x, int y) { return x | y; });
   double S = 0.0;
@@ -770,6 +799,7 @@ Args rows_from(const Args& a, int64_t r0, int64_t rows) {
   if (a.stats_in) b.stats_in = a.stats_in + r0;
   if (a.stats_out) b.stats_out = a.stats_out + r0;
   if (a.dz) b.dz = static_cast<TO*>(a.dz) + r0 * a.ldd;
+  if (a.near) b.near = a.near + r0;
   return b;
 }
 
@@ -840,9 +870,13 @@ void launch_resident(const Args& a, hipStream_t stream) {
 
 template <class T, class TO>
 void run_rows(Args a, RowStats* ws, hipStream_t stream) {
-  if (a.T > HOT_T) return launch_hot<T, TO>(a, stream);
   const Plan p = make_plan<T>(a.B, a.K);
-  if (p.parts == 0) return launch_resident<T, TO>(a, stream);
+  a.find = true;
+  if (p.parts == 0) {
+    launch_resident<T, TO>(a, stream);
+    if (a.near != nullptr) launch_hot<T, TO>(a, stream);
+    return;
+  }
   const size_t lds = Listed::bytes(a.k, a.K);
   a.parts = 1;
   for (int64_t r0 = 0; r0 < a.B; r0 += 65535) {  // grid.y holds 16 bits
@@ -854,15 +888,19 @@ void run_rows(Args a, RowStats* ws, hipStream_t stream) {
       b.stats_in = ws + r0 * p.parts;
       b.parts = p.parts;
     }
-    // the loss gathers logits of the whole row: where the gradient overwrites them it goes first
-    if (b.dz == b.Z && b.loss != nullptr) {
+    // the loss gathers logits of the whole row, and so does the search for near rows: where the gradient overwrites
+    // them, or leaves such rows out, they go first
+    const bool first = b.near != nullptr || (b.dz == b.Z && b.loss != nullptr);
+    if (first) {
       Args l = b;
       l.dz = nullptr;
       hipLaunchKernelGGL((distill_chunks_kernel<T, TO>), dim3(1, rows), dim3(PART_THREADS), lds, stream, l, p.len);
-      b.loss = nullptr;
+      b.loss = nullptr, b.find = false;
     }
-    hipLaunchKernelGGL((distill_chunks_kernel<T, TO>), dim3(b.dz == nullptr ? 1u : (unsigned)p.parts, rows),
-                       dim3(PART_THREADS), lds, stream, b, p.len);
+    if (!first || b.dz != nullptr)
+      hipLaunchKernelGGL((distill_chunks_kernel<T, TO>), dim3(b.dz == nullptr ? 1u : (unsigned)p.parts, rows),
+                         dim3(PART_THREADS), lds, stream, b, p.len);
+    if (b.near != nullptr) launch_hot<T, TO>(rows_from<T, TO>(a, r0, rows), stream);
   }
   MLAPI_HIP_CHECK(hipGetLastError());
 }
@@ -875,10 +913,14 @@ void run_distill(const Args& a, RowStats* ws, hipStream_t stream) {
 
 }  // namespace
 
-size_t distill_workspace(int dt, int64_t B, int K) {
+namespace {
+size_t near_bytes(int64_t B, float T) { return T > HOT_T ? ((size_t)B * sizeof(int32_t) + 15) / 16 * 16 : 0; }
+}  // namespace
+
+size_t distill_workspace(int dt, int64_t B, int K, float temperature, bool stats_given) {
   if (B <= 0 || K < 1) return 0;
   const Plan p = dt == DT_F32 ? make_plan<float>(B, K) : make_plan<__bf16>(B, K);
-  return (size_t)p.parts * (size_t)B * sizeof(RowStats);
+  return near_bytes(B, temperature) + (stats_given ? 0 : (size_t)p.parts * (size_t)B * sizeof(RowStats));
 }
 
 void launch_distill(const DistillCall& c, hipStream_t stream) {
@@ -891,7 +933,7 @@ void launch_distill(const DistillCall& c, hipStream_t stream) {
   if (!(c.alpha >= 0.f && c.alpha <= 1.f)) throw std::invalid_argument("distill: alpha in [0, 1]");
   if (c.ldz < c.K || (c.dz != nullptr && c.ldd < c.K)) throw std::invalid_argument("distill: row stride below K");
   if (c.alpha != 1.f && c.y == nullptr) throw std::invalid_argument("distill: alpha below 1 needs labels");
-  if (c.stats_in == nullptr && c.ws_bytes < distill_workspace(c.dt, c.B, c.K))
+  if (c.ws_bytes < distill_workspace(c.dt, c.B, c.K, c.temperature, c.stats_in != nullptr))
     throw std::invalid_argument("distill: workspace too small");
   Args a{};
   a.Z = c.Z, a.idx = c.idx, a.t = c.t, a.y = c.y, a.g = c.g, a.loss = c.loss, a.dz = c.dz, a.pred = c.pred;
@@ -901,7 +943,9 @@ void launch_distill(const DistillCall& c, hipStream_t stream) {
   a.K = c.K, a.k = c.k, a.parts = 1, a.t_dt = c.t_dt;
   a.T = c.temperature, a.soft = c.alpha, a.hard = c.y != nullptr ? 1.f - c.alpha : 0.f;
   a.two = a.hard != 0.f && c.temperature != 1.f;
-  RowStats* ws = static_cast<RowStats*>(c.workspace);
+  const size_t near = near_bytes(c.B, c.temperature);
+  a.near = near != 0 ? static_cast<int32_t*>(c.workspace) : nullptr;
+  RowStats* ws = reinterpret_cast<RowStats*>(static_cast<char*>(c.workspace) + near);
   if (c.dt == DT_F32 && c.out_dt == DT_F32) return run_distill<float, float>(a, ws, stream);
   if (c.dt == DT_F32 && c.out_dt == DT_BF16) return run_distill<float, __bf16>(a, ws, stream);
   if (c.dt == DT_BF16 && c.out_dt == DT_BF16) return run_distill<__bf16, __bf16>(a, ws, stream);

@@ -61,7 +61,7 @@ Layout make_layout(int64_t B, int K, int F) {
   L.stats = take((size_t)L.stat_blocks * 2 * sizeof(float));
   L.loss = take((size_t)B * sizeof(float));
   L.pred = take((size_t)B * sizeof(int32_t));
-  L.rows = take(distill_workspace(DT_F32, B, K));
+  L.rows = take(distill_workspace(DT_F32, B, K, 1e6f));  // enough for every temperature
   L.total = o;
   return L;
 }

@@ -178,7 +178,7 @@ def _distill(name: str, Z, idx, t, temperature, alpha, y, *, g=None, stats_in=No
     stats = torch.empty((B, 4), dtype=torch.float32, device=dev) if stats else None
     c = C()
     with _On(Z) as stream:
-        n = 0 if stats_in is not None else c.distill_workspace(dt, B, K)
+        n = c.distill_workspace(dt, B, K, temperature, stats_in is not None)
         ws, at = _workspace(n, dev)
         c.distill(dt, _DT[t.dtype], ddt, Z.data_ptr(), ld, B, K, idx.data_ptr(), idx.stride(0) if B > 1 else k,
                   t.data_ptr(), t.stride(0) if B > 1 else k, k, temperature, alpha, yp, gp,
@@ -197,7 +197,8 @@ def distill_loss(Z: torch.Tensor, idx: torch.Tensor, t: torch.Tensor, *, tempera
 
         loss = alpha T^2 sum_j q_j (ln q_j - ln p[idx_j])  -  (1 - alpha) ln softmax(Z)[y]        (f32 [B])
 
-    T in [1e-6, 1e6]; above 16, where T^2 would count what 32-bit sums are off, sums and loss are evaluated in 64 bits.
+    T in [1e-6, 1e6]; above 16, where T^2 would count what 32-bit sums are off, a row whose list holds nearly all of p is
+    evaluated in 64 bits.
     A row without entries has no first part, a row with y < 0 no second, a row whose logits are all -inf
     neither. A listed class that the student masks makes the loss +inf. A class >= K in idx or y makes its
     row's loss and gradient NaN."""
