@@ -289,6 +289,36 @@ def test_trainer_steps_on_the_gpu_follow_the_cpu_ones_and_a_captured_step_the_ea
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k", [5, 77])
+def test_gradient_at_a_high_temperature(k):
+    """Lists of some classes and of all: rows that take 32 bits, and 64, of one workspace."""
+    from mlapi_amd.ops import linear as ops
+
+    B, F, K, T, alpha, u = 300, 128, 77, 40.0, 0.6, 2.0 ** -24
+    g = torch.Generator().manual_seed(k)
+    Xa = ops.augment_features(torch.randn(B, F, generator=g).to("cuda:0"), F + 8)
+    W = (torch.randn(K, F, generator=g) / F ** 0.5).to(torch.bfloat16).to("cuda:0")
+    b = (0.1 * torch.randn(K, generator=g)).to("cuda:0")
+    y = torch.randint(0, K, (B,), generator=g).to(torch.int32).to("cuda:0")
+    Wa = torch.cat([W.double(), b.double()[:, None], torch.zeros(K, 7, device="cuda:0", dtype=torch.float64)], 1)
+    z = Xa.double() @ Wa.T
+    t, idx = torch.topk(z + 0.5 * torch.randn(B, K, generator=g, dtype=torch.float64).to("cuda:0"), k, dim=1)
+    idx, t = idx.to(torch.int32), t.float()
+    how = dict(temperature=T, alpha=alpha, y=y)
+    dW, stats = ops.softmax_distill_grad(Xa, W, b, idx, t, **how)
+    G, rdW, loss, _ = ref.softmax_distill_ref(Xa, Wa, idx, t, **how, dtype=torch.float64)
+    # z is off by F + 1 f32 products; G then by as much (its slope is below 1), by a row's f32 sums (none in the soft part
+    # where the list is whole, whose p and q are 64-bit) and by its rounding to bf16; then a sum over B rows
+    ez = (F + 2) * u * (Xa.double().abs() @ Wa.abs().T).max()
+    eG = G.abs() * 2.0 ** -8 + 2 * ez + 40 * u * (T if k < K else 1.0)
+    tol = eG.T @ Xa.double().abs() + (B + 64) * u * (G.abs().T @ Xa.double().abs())
+    assert ((dW.double() - rdW).abs() <= tol).all(), ((dW.double() - rdW).abs() - tol).max()
+    # the loss moves by its gradient, sum |G| <= 2 a T + 2 of it at most, with z; its f32 sums count T^2 in the soft part
+    tol = B * ((2 * alpha * T + 2) * ez.item() + 40 * u * (T * T if k < K else 8.0)) + 400 * u * loss.item()
+    assert abs(stats[0].item() - loss.item()) <= tol and (k < K or tol < 0.1 * loss.item())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("momentum", [0.0, 0.9])
 def test_every_trainer_step_on_the_gpu_is_the_plain_one(momentum):
     """Each step against 64 bits from the weights, shadows and momenta before it, to a bound that the step is far above."""
